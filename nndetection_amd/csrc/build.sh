@@ -1,9 +1,11 @@
 #!/bin/bash
-# Build libnndet_amd.so for gfx950 (cross-compiles without a GPU). Usage: csrc/build.sh [-j N]
+# Build libnndet_amd.so for gfx950 (cross-compiles without a GPU). Usage: csrc/build.sh; REBUILD=1 compiles every source again
 set -e
 cd "$(dirname "$0")"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
-COMMON="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wno-unused-result"
+# -packed-fp32-ops: hipcc -O3 makes v_pk_{add,mul,fma}_f32 out of ordinary float code, and some of their forms have given wrong results
+# on this part without any error; scalar fp32 instructions only. (The host pass warns that it does not know the feature: harmless.)
+COMMON="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p _obj
 pids=()
 # build.sh --asm DIR : emit the gfx950 ISA of every source (same flags) into DIR/*.s instead of building the library
@@ -18,7 +20,7 @@ build() { # src extra-flags
     return
   fi
   local obj=_obj/${src%.hip}.o
-  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ common.h -nt "$obj" ] || [ conv_common.h -nt "$obj" ] || [ radix_select.h -nt "$obj" ] || [ ../../include/nndet_amd.h -nt "$obj" ]; then
+  if [ -n "$REBUILD" ] || [ ! -f "$obj" ] || [ build.sh -nt "$obj" ] || [ "$src" -nt "$obj" ] || [ common.h -nt "$obj" ] || [ conv_common.h -nt "$obj" ] || [ radix_select.h -nt "$obj" ] || [ ../../include/nndet_amd.h -nt "$obj" ]; then
     $HIPCC $COMMON "$@" -c "$src" -o "$obj" &
     pids+=($!)
   fi
