@@ -473,13 +473,15 @@ for _kv in os.environ.get("NNDET_STREAM_PADS", "").split(","):
 _pad_streams = []          # (kept alive: a destroyed stream gives its queue reference back)
 
 
-def new_stream(kind: str, device, priority: int = 0):
+def new_stream(kind: str, device):
+    """A side stream of the package, at the default priority like every stream here: work on streams of DIFFERENT priorities has hung for
+    good on this part."""
     for _ in range(_STREAM_PADS.pop(kind, 0)):               # (once per kind)
-        ps = torch.cuda.Stream(device=device, priority=priority)
+        ps = torch.cuda.Stream(device=device)
         with torch.cuda.stream(ps):
             torch.zeros(1, device=device)                    # first use binds the hardware queue
         _pad_streams.append(ps)
-    return torch.cuda.Stream(device=device, priority=priority)
+    return torch.cuda.Stream(device=device)
 
 
 class _WgradStreams:
@@ -526,14 +528,11 @@ class _WgradStreams:
         idx = dev.index if dev.index is not None else torch.cuda.current_device()
         ws = self.streams.get(idx)
         if ws is None:
-            # lowest queue priority the device offers: the critical chain on the other streams gets the CUs first, the weight
-            # gradients take what is left (NNDET_WGRAD_PRIO overrides: -1 high, 0 normal, 1 low on ROCm)
-            prio = int(os.environ.get("NNDET_WGRAD_PRIO", "1"))
             mask = os.environ.get("NNDET_WGRAD_CUMASK", "")
             if mask:
                 ws = self.streams[idx] = cumask_stream(dev, mask)
             else:
-                ws = self.streams[idx] = new_stream("wgrad", dev, prio)
+                ws = self.streams[idx] = new_stream("wgrad", dev)
         return ws
 
     def _done(self):

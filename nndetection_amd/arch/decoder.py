@@ -96,7 +96,7 @@ class UFPNModular(nn.Module):
         if level == 0 and self.split_tail and self.num_level >= 3 and need0:
             side = UFPNModular._tail_streams.get(dev.index or 0)        # level 0 stays on the tail stream of forward()
             if side is None:
-                side = UFPNModular._tail_streams[dev.index or 0] = L.new_stream("tail", dev, int(os.environ.get("NNDET_PRIO_TAIL", "0")))
+                side = UFPNModular._tail_streams[dev.index or 0] = L.new_stream("tail", dev)
         else:
             side = UFPNModular._early_streams.get(dev.index or 0)
             if side is None:
@@ -134,7 +134,7 @@ class UFPNModular(nn.Module):
             main = torch.cuda.current_stream(dev)
             side = UFPNModular._tail_streams.get(dev.index or 0)
             if side is None:
-                side = UFPNModular._tail_streams[dev.index or 0] = L.new_stream("tail", dev, int(os.environ.get("NNDET_PRIO_TAIL", "0")))
+                side = UFPNModular._tail_streams[dev.index or 0] = L.new_stream("tail", dev)
             if fpn[0] is None and not absorb:
                 side.wait_stream(main)                           # the encoder outputs are ready
                 inp_seq[0].record_stream(side)

@@ -135,7 +135,7 @@ class BaseRetinaNet(nn.Module):
             elif kind == "tail" and isinstance(self.decoder, UFPNModular) and self.decoder.split_tail:
                 st = UFPNModular._tail_streams.get(idx)
                 if st is None:
-                    st = UFPNModular._tail_streams[idx] = L.new_stream("tail", device, int(os.environ.get("NNDET_PRIO_TAIL", "0")))
+                    st = UFPNModular._tail_streams[idx] = L.new_stream("tail", device)
             elif kind == "head" and hasattr(self.head, "_side_streams") and getattr(self.head, "multi_stream", False):
                 st = self.head._side_streams(device, 1)[0]
             elif kind == "wgrad" and L.wgrad_streams.enabled:
@@ -306,7 +306,7 @@ class BaseRetinaNet(nn.Module):
     def _aux(self, device, i: int):
         pool = BaseRetinaNet._aux_streams.setdefault(device.index or 0, [])
         while len(pool) <= i:
-            pool.append(L.new_stream("aux%d" % len(pool), device, int(os.environ.get("NNDET_PRIO_AUX%d" % len(pool), os.environ.get("NNDET_PRIO_AUX", "0")))))
+            pool.append(L.new_stream("aux%d" % len(pool), device))
         return pool[i]
 
     # ------------------------------------------------------------------ train step (retina.py:86-159)

@@ -1,18 +1,17 @@
 #!/usr/bin/env python
 """How the step time depends on which hardware queue a side stream lands on.  HIP maps streams onto GPU_MAX_HW_QUEUES (default 4) hardware
 queues when they are created / first used; D dummy streams created (and touched) BEFORE the framework creates its own shift that mapping.
-  tools/stream_map_probe.py D [prio ...]      D dummies of normal priority, then optional extra dummies of the given priorities
+  tools/stream_map_probe.py D      D dummies
 Prints ms per step (60 steps after 15 warm-up, batch 4 bf16 luna160)."""
 import os, sys, time
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch
 D = int(sys.argv[1]) if len(sys.argv) > 1 else 0
-extra = [int(a) for a in sys.argv[2:]]
 dev = torch.device("cuda:0")
 torch.cuda.init()
 keep = []
-for pr in [0] * D + extra:
-    s = torch.cuda.Stream(device=dev, priority=pr)
+for _ in range(D):
+    s = torch.cuda.Stream(device=dev)
     with torch.cuda.stream(s):
         torch.zeros(1, device=dev)
     keep.append(s)
