@@ -693,6 +693,49 @@ int nndet_detloss_matched_f32(const float* logits, const float* deltas, int32_t 
                               int32_t C, float eps, float clip, float reg_weight, int32_t reg_mean, float cls_weight, int32_t cls_mean,
                               float* losses_out, float* g_deltas_out, float* g_logits_out, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Optimiser step over many tensors at once (csrc/optim.hip). The reference builds torch.optim.SGD
+ * (nndet/ptmodule/retinaunet/base.py:313-322) and leaves clipping to the trainer; these entries give the AdamW step, the global
+ * gradient norm with clipping, and AdamW with 8-bit moments to a training loop on the same network.
+ *
+ * A tensor of a call (host memory; the pointers in it are device pointers). Elements are taken in the order of the memory: param,
+ * grad and the moments of a tensor have the same order, and no two tensors of a call overlap. Any alignment of whole elements is
+ * accepted; tensors whose pointers are 16-B aligned take the vector path. numel 0 is allowed (its step count still advances).
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct NndetOptTensor {
+    void* param;            /* [numel] of dtype; nndet_adam_state8: fp32 exp_avg */
+    void* grad;             /* [numel] of dtype; nndet_adam_state8: fp32 exp_avg_sq */
+    void* exp_avg;          /* state_bits 32: fp32 [numel]; 8: e4m3 codes [numel] */
+    void* exp_avg_sq;       /* state_bits 32: fp32 [numel]; 8: e4m3 codes [numel] of its SQUARE ROOT */
+    float* exp_avg_scale;   /* state_bits 8: [ceil(numel / 256)] scale of each 256 consecutive elements */
+    float* root_scale;      /* state_bits 8: the same for the square roots */
+    int64_t numel;          /* < 2^40 */
+    double weight_decay;    /* decoupled: param *= 1 - lr * weight_decay */
+    int32_t slot;           /* its step count is steps[slot]; 0 <= slot < 2^24, no slot twice in a call */
+    int16_t dtype;          /* NNDET_F32 / NNDET_BF16 / NNDET_F16 of param and grad */
+    int16_t state_bits;     /* 32 or 8 */
+} NndetOptTensor;
+typedef struct NndetAdamw {
+    double lr, beta1, beta2, eps;
+    double max_norm;            /* >= 0: multiply the gradients by min(1, max_norm / (norm + 1e-6)) on the way; < 0: no clipping */
+    const float* lr_device;     /* not NULL: the rate is read there instead (a captured step follows a schedule) */
+    const float* grad_scale;    /* not NULL: the gradients carry this loss scale (torch.amp.GradScaler); they are divided by it */
+    const float* found_inf;     /* not NULL and not 0 on the device: nothing but norm is written */
+    float* norm;                /* max_norm >= 0: [1] global 2-norm of the gradients without their scale, written (or NULL), or ... */
+    int64_t norm_given;         /* ... not 0: read instead of computed (a norm over more tensors than this call's) */
+    int32_t* steps;             /* step counts, advanced on the device */
+} NndetAdamw;
+/* Device bytes (16-B aligned) that the three calls below need for n tensors; free again when the call's work is done. */
+size_t nndet_opt_workspace_bytes(int32_t n);
+/* One AdamW step (torch.optim.AdamW's formula, each operation rounded to fp32) of all tensors, moments in 32 or 8 bits as each tensor says. */
+int nndet_adamw_step(const NndetOptTensor* tensors, int32_t n, const NndetAdamw* args, void* workspace, size_t workspace_bytes, void* stream);
+/* norm_out[0] = 2-norm over the gradients of all tensors (squares summed in fp64), divided by *grad_scale if that is not NULL;
+ * max_norm >= 0: the gradients are multiplied in place by min(1, max_norm / (norm + 1e-6)) (torch.nn.utils.clip_grad_norm_; grad_scale
+ * NULL); max_norm < 0: the norm alone. */
+int nndet_grad_clip(const NndetOptTensor* tensors, int32_t n, double max_norm, const float* grad_scale, float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+/* write != 0: fp32 moments (in param, grad) to 8 bits (in exp_avg .. root_scale), rounded to nearest even; write == 0: back. */
+int nndet_adam_state8(const NndetOptTensor* tensors, int32_t n, int32_t write, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -49,6 +49,19 @@ class NndetItems(C.Structure):
                 ("dims", (C.c_int32 * 3) * MAX_ITEMS), ("row_off", C.c_int64 * MAX_ITEMS)]
 
 
+class NndetOptTensor(C.Structure):
+    """One tensor of an optimiser call. The calls fill it as nine 64-bit words (`_words` in optim.py), this is its layout."""
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("exp_avg_scale", C.c_void_p), ("root_scale", C.c_void_p), ("numel", C.c_int64), ("weight_decay", C.c_double),
+                ("slot", C.c_int32), ("dtype", C.c_int16), ("state_bits", C.c_int16)]
+
+
+class NndetAdamw(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("max_norm", C.c_double),
+                ("lr_device", C.c_void_p), ("grad_scale", C.c_void_p), ("found_inf", C.c_void_p), ("norm", C.c_void_p),
+                ("norm_given", C.c_int64), ("steps", C.c_void_p)]
+
+
 _P, _I64, _I32, _F, _SZ = C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_size_t
 _CONVP = C.POINTER(NndetConv)
 _ITEMSP = C.POINTER(NndetItems)
@@ -154,6 +167,10 @@ SIGNATURES = {
                                                _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "nndet_conv_out_sparse_backward": (C.c_int, [_CONVP, _ITEMSP, _P, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _P]),
     "nndet_segloss_tail_f32": (C.c_int, [_P, _I64, _F, _F, _F, _P, _P, _P]),
+    "nndet_opt_workspace_bytes": (_SZ, [_I32]),
+    "nndet_adamw_step": (C.c_int, [_P, _I32, C.POINTER(NndetAdamw), _P, _SZ, _P]),
+    "nndet_grad_clip": (C.c_int, [_P, _I32, C.c_double, _P, _P, _P, _SZ, _P]),
+    "nndet_adam_state8": (C.c_int, [_P, _I32, _I32, _P, _SZ, _P]),
     "nndet_sigmoid_max_f32": (C.c_int, [_P, _I64, _I32, _P, _P]),
 }
 

@@ -45,6 +45,7 @@ build segloss.hip
 build headio.hip
 build sparse_out.hip
 build segbranch.hip
+build optim.hip -ffp-contract=off
 build api.hip
 rc=0
 for p in "${pids[@]}"; do wait $p || rc=1; done

@@ -1,15 +1,24 @@
-"""Lean SGD(nesterov) + LinearWarmupPolyLR for the training step.
+"""Optimisers of the training step: lean SGD(nesterov), AdamW with moments in 32 or in 8 bits, clipping by the global gradient norm, and
+LinearWarmupPolyLR.
 
-Same update rule as `torch.optim.SGD(momentum, nesterov, weight_decay)` as configured by the reference
+SGD: same update rule as `torch.optim.SGD(momentum, nesterov, weight_decay)` as configured by the reference
 (nndet/ptmodule/retinaunet/base.py:300-336) and the same per-iteration schedule as `LinearWarmupPolyLR`
 (nndet/training/learning_rate.py:26-57,127-184), but issued as a handful of `torch._foreach_*` launches over static
 tensor lists: torch.optim's per-step Python bookkeeping cost ~5 ms of GPU idle time per step after backward
 (profiles/round1_v2_kernel_stats.txt gap analysis), which is 10 % of the whole step at MI355X speed.
+
+AdamW and clipping: HIP kernels over all tensors of a call at once (csrc/optim.hip). `AdamW` is the optimiser; `adamw_step`, `adamw8_step`,
+`grad_norm`, `clip_grads_`, `write_adam_state8` and `read_adam_state8` are the same operators on lists of tensors. They run on torch's
+current stream of the tensors' device, never wait for the GPU, and can be captured into a HIP graph.
 """
+import array
 import os
-from typing import List
+import struct
+from typing import List, NamedTuple, Optional, Sequence, Union
 
 import torch
+
+from . import _lib as L
 
 
 def _bump_versions(tensors) -> None:
@@ -137,10 +146,498 @@ class SGDNesterov:
                     p.grad.zero_()
 
 
+# ---- operators over lists of tensors ------------------------------------------------------------------------------------------------
+
+STATE8_BLOCK = 256                                   # consecutive elements of a tensor that share one scale of the 8-bit moments
+_F8 = torch.float8_e4m3fn
+
+
+class AdamState8(NamedTuple):
+    """AdamW moments in 8 bits, one entry a tensor in every list. exp_avg / root: float8_e4m3fn codes in the parameter's shape and memory
+    order, of the first moment and of the SQUARE ROOT of the second; exp_avg_scale / root_scale: fp32, one value for each STATE8_BLOCK
+    consecutive elements (in memory order). A moment is code * scale."""
+    exp_avg: Sequence[torch.Tensor]
+    exp_avg_scale: Sequence[torch.Tensor]
+    root: Sequence[torch.Tensor]
+    root_scale: Sequence[torch.Tensor]
+
+    @staticmethod
+    def zeros(params: Sequence[torch.Tensor]) -> "AdamState8":
+        """The state before the first step of `params`."""
+        codes = lambda: [torch.zeros_like(p, dtype=torch.uint8).view(_F8) for p in params]  # noqa: E731
+        scales = lambda: [torch.zeros((-(-p.numel() // STATE8_BLOCK),), dtype=torch.float32, device=p.device) for p in params]  # noqa: E731
+        return AdamState8(codes(), scales(), codes(), scales())
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Do the elements fill one piece of memory, in any order of the dimensions, each place once?"""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != size:
+            return False
+        size *= n
+    return True
+
+
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Have two dense tensors of one shape the same memory order?"""
+    return all(x == y or n == 1 for x, y, n in zip(a.stride(), b.stride(), a.shape)) or a.numel() == 0
+
+
+def _refuse(what: str):
+    raise L.NndetError(what)
+
+
+def _check_list(name: str, ts, dtype, device, like=None) -> None:
+    """Tensors of one type on one GPU, dense; `like`: and of the same sizes and memory order, one for one."""
+    for i, t in enumerate(ts):
+        if t.device != device:
+            _refuse(f"{name}[{i}] is on {t.device}, not on {device}: the tensors of a call are on one GPU")
+        if dtype is not None and t.dtype != dtype:
+            _refuse(f"{name}[{i}] is {t.dtype}, not {dtype}")
+        if like is not None:
+            p = like[i]
+            if t.shape != p.shape:
+                _refuse(f"{name}[{i}] has shape {tuple(t.shape)}, the parameter {tuple(p.shape)}")
+            if not (t.is_contiguous() and p.is_contiguous()) and not (_dense(t) and _same_order(t, p)):
+                _refuse(f"{name}[{i}] has strides {t.stride()}, the parameter {p.stride()}: moments lie in the parameter's memory order")
+        elif not _dense(t):
+            _refuse(f"{name}[{i}] with strides {t.stride()} is not dense in memory")
+
+
+def _check_lengths(n: int, **lists) -> None:
+    for name, ts in lists.items():
+        if len(ts) != n:
+            _refuse(f"{len(ts)} {name} for {n} tensors")
+
+
+def _check_distinct(name: str, ts) -> None:
+    ptrs = [t.data_ptr() for t in ts if t.numel()]
+    if len(set(ptrs)) != len(ptrs):
+        _refuse(f"the same tensor twice in {name}: its updates would race")
+
+
+def _scalar(name: str, t, device) -> Optional[int]:
+    """Address of a one-element fp32 tensor on `device`, None for None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+        _refuse(f"{name} is one fp32 value on {device}")
+    return t.data_ptr()
+
+
+_KIND = {torch.float32: L.F32 << 32, torch.bfloat16: L.BF16 << 32, torch.float16: L.F16 << 32}
+
+
+def _kinds(ts) -> list:
+    try:
+        return [_KIND[t.dtype] for t in ts]
+    except KeyError as e:
+        raise L.NndetError(f"unsupported type {e.args[0]}; use float32, bfloat16 or float16")
+
+
+def _double_bits(x: float) -> int:
+    return struct.unpack("q", struct.pack("d", x))[0]
+
+
+def _words(n, p, g, m, v, ms, rs, numel, wd, tail) -> array.array:
+    """The call's tensors as NndetOptTensor structs (nine 64-bit words each). p .. rs: lists of addresses or None, wd: the bits of doubles or
+    None, tail: slot | type << 32 | bits of the moments << 48."""
+    zero = [0] * n
+    rows = zip(p or zero, g or zero, m or zero, v or zero, ms or zero, rs or zero, numel, wd or zero, tail)
+    return array.array("q", [w for row in rows for w in row])
+
+
+def _run(device, what: str, words, n: int, *args) -> None:
+    """Call `what`(tensors, n, *args, workspace, bytes, stream) on the device's current stream, with a workspace of this call."""
+    if device.type != "cuda":
+        _refuse(f"tensors on {device}: nndetection_amd kernels need tensors on the GPU (no CPU path)")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _run(device, what, words, n, *args)
+    nbytes = L.load().nndet_opt_workspace_bytes(n)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    L.call(what, words.buffer_info()[0], n, *args, ws.data_ptr(), nbytes, L.stream())
+
+
+def _ptrs(ts) -> list:
+    return [t.data_ptr() for t in ts]
+
+
+def _written(ts) -> None:
+    """The kernels write through raw pointers: advance the version counters as torch's in-place operators do."""
+    if ts:
+        try:
+            _bump_versions(ts)
+        except RuntimeError:                         # inference tensors have no version counter
+            pass
+
+
+def _grads_like(params, grads) -> list:
+    """Gradients in the parameters' memory order (a copy where they are not)."""
+    out = []
+    for i, (p, g) in enumerate(zip(params, grads)):
+        if g.is_sparse or g.shape != p.shape:
+            _refuse(f"grads[{i}] is {'sparse' if g.is_sparse else 'of shape %s' % (tuple(g.shape),)}, the parameter is dense {tuple(p.shape)}")
+        if g.dtype != p.dtype or g.device != p.device:
+            _refuse(f"grads[{i}] is {g.dtype} on {g.device}, the parameter {p.dtype} on {p.device}")
+        if not (g.is_contiguous() and p.is_contiguous()) and not (_dense(g) and _same_order(g, p)):
+            g = torch.empty_like(p).copy_(g.detach())
+        out.append(g)
+    return out
+
+
+Rate = Union[float, torch.Tensor]
+
+
+def _hyper(lr, betas, eps, max_norm, total_norm, grad_scale, found_inf, steps, device):
+    """The scalars of a step as the library takes them, checked, and the norm's tensor (None without clipping)."""
+    b1, b2 = float(betas[0]), float(betas[1])
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
+        _refuse(f"betas {betas} in [0, 1) and eps {eps} >= 0 are wanted")
+    if max_norm is not None and not max_norm >= 0.0:
+        _refuse(f"max_norm {max_norm} >= 0 is wanted")
+    if total_norm is not None and max_norm is None:
+        _refuse("total_norm without max_norm")
+    norm = total_norm
+    if max_norm is not None and norm is None:
+        norm = torch.empty((), dtype=torch.float32, device=device)
+    rate = 0.0
+    if not isinstance(lr, torch.Tensor):
+        lr, rate = None, float(lr)
+    elif lr.device.type == "cpu" and device.type != "cpu":
+        lr, rate = None, float(lr)
+    a = L.NndetAdamw(rate, b1, b2, float(eps), -1.0 if max_norm is None else float(max_norm), _scalar("lr", lr, device),
+                     _scalar("grad_scale", grad_scale, device), _scalar("found_inf", found_inf, device), _scalar("total_norm", norm, device),
+                     int(total_norm is not None), steps.data_ptr())
+    return a, norm
+
+
+def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight_decay, max_norm, total_norm, grad_scale, found_inf):
+    n = len(params)
+    _check_lengths(n, grads=grads, exp_avgs=m, exp_avg_sqs=v)
+    if not isinstance(steps, torch.Tensor) or steps.dtype != torch.int32 or steps.dim() != 1 or not steps.is_contiguous() or steps.numel() < n:
+        _refuse(f"steps is one int32 count a tensor ({n}), contiguous")
+    wd = weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+    _check_lengths(n, weight_decay=wd)
+    slots = range(n)
+    if any(g is None for g in grads):                # these tensors and their counts stay as they are
+        slots = [i for i, g in enumerate(grads) if g is not None]
+        pick = lambda ts: None if ts is None else [ts[i] for i in slots]  # noqa: E731
+        params, grads, m, v, ms, rs, wd = (pick(x) for x in (params, grads, m, v, ms, rs, wd))
+        n = len(params)
+    device = steps.device
+    _check_list("params", params, None, device)
+    grads = _grads_like(params, grads)
+    kinds = _kinds(params)
+    for name, ts in (("exp_avgs", m), ("exp_avg_sqs", v)):
+        _check_list(name, ts, torch.float32 if bits == 32 else _F8, device, params)
+    numel = [p.numel() for p in params]
+    if bits == 8:
+        for name, ts in (("exp_avg_scale", ms), ("root_scale", rs)):
+            _check_scales(name, ts, numel, device)
+    _check_distinct("params and moments", [*params, *m, *v])
+    a, norm = _hyper(lr, betas, eps, max_norm, total_norm, grad_scale, found_inf, steps, device)
+    bits_of = {w: _double_bits(float(w)) for w in set(wd)}
+    words = _words(n, _ptrs(params), _ptrs(grads), _ptrs(m), _ptrs(v), ms and _ptrs(ms), rs and _ptrs(rs), numel, [bits_of[w] for w in wd],
+                   [s | k | (bits << 48) for s, k in zip(slots, kinds)])
+    _run(device, "nndet_adamw_step", words, n, L.C.byref(a))
+    _written(params)
+    return norm
+
+
+def _check_scales(name: str, ts, numel, device) -> None:
+    for i, (t, n) in enumerate(zip(ts, numel)):
+        if t.dtype != torch.float32 or t.device != device or t.numel() != -(-n // STATE8_BLOCK) or not t.is_contiguous():
+            _refuse(f"{name}[{i}] is one fp32 value on {device} for each {STATE8_BLOCK} elements of the tensor ({-(-n // STATE8_BLOCK)}), contiguous")
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps: torch.Tensor, *, lr: Rate, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay=0.01, max_norm: Optional[float] = None, total_norm: Optional[torch.Tensor] = None,
+               grad_scale: Optional[torch.Tensor] = None, found_inf: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """One AdamW step of many tensors in place (torch.optim.AdamW's formula):
+
+        t = steps + 1;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    params / grads: fp32, bf16 or fp16 tensors (any mixture) on one GPU, dense in memory; a gradient in another memory order is copied
+    first, a gradient None leaves its tensor, moments and count as they are. exp_avgs / exp_avg_sqs: fp32, in the parameters' memory order.
+    steps: int32 counts on the GPU, one a tensor. No two of the tensors may overlap. lr: a number, or one fp32 value on the GPU (a captured
+    step follows a schedule through it). weight_decay: a number, or one a tensor.
+    max_norm: the gradients are multiplied by min(1, max_norm / (norm + 1e-6)) on the way (they are not written), where norm is `total_norm`
+    or else the 2-norm over all gradients of the call; the norm is returned, on the GPU. A norm that is not finite gives what it gives in
+    torch's clipping: NaN. grad_scale: the gradients carry this loss scale and are divided by it, before the norm. found_inf: where it is
+    not 0 nothing is changed (torch.amp.GradScaler hands both over)."""
+    return _adamw_call(params, grads, exp_avgs, exp_avg_sqs, None, None, 32, steps, lr, betas, eps, weight_decay, max_norm, total_norm,
+                       grad_scale, found_inf)
+
+
+def adamw8_step(params, grads, state: AdamState8, steps: torch.Tensor, *, lr: Rate, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01,
+                max_norm: Optional[float] = None, total_norm: Optional[torch.Tensor] = None, grad_scale: Optional[torch.Tensor] = None,
+                found_inf: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """`adamw_step` with the moments in 8 bits: 2.03 bytes an element instead of 8. The step itself is computed in fp32 from the moments as
+    they are stored; the new ones are then rounded, the first to the nearest code, the root of the second up or down with the probability
+    that keeps its expected value (by bits that follow from the element's index and its step count: the same step gives the same state).
+    A gradient that is not finite makes the moments of its whole block NaN; `found_inf` keeps it out."""
+    m, ms, v, rs = state
+    _check_lengths(len(params), exp_avg_scale=ms, root_scale=rs)
+    return _adamw_call(params, grads, m, v, ms, rs, 8, steps, lr, betas, eps, weight_decay, max_norm, total_norm, grad_scale, found_inf)
+
+
+def _clip_call(grads, max_norm: float, grad_scale) -> torch.Tensor:
+    n = len(grads)
+    for i, g in enumerate(grads):
+        if g.is_sparse:
+            _refuse(f"grads[{i}] is sparse")
+    device = grads[0].device if n else torch.device("cuda", torch.cuda.current_device())
+    kinds = _kinds(grads)
+    flat = [g if _dense(g) else g.contiguous() for g in grads]
+    _check_list("grads", flat, None, device)
+    if max_norm >= 0.0:
+        _check_distinct("grads", grads)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    words = _words(n, None, _ptrs(flat), None, None, None, None, [g.numel() for g in flat], None, [k | (32 << 48) for k in kinds])
+    _run(device, "nndet_grad_clip", words, n, max_norm, _scalar("grad_scale", grad_scale, device), norm.data_ptr())
+    if max_norm >= 0.0:
+        _written(flat)
+        for g, f in zip(grads, flat):
+            if f is not g:
+                g.copy_(f)
+    return norm
+
+
+def grad_norm(grads, grad_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """2-norm over all `grads` (fp32, bf16 or fp16 on one GPU; squares are summed in fp64) as one fp32 value on the GPU; divided by
+    `grad_scale`, one fp32 value there, if they carry a loss scale."""
+    return _clip_call([g for g in grads if g is not None], -1.0, grad_scale)
+
+
+def clip_grads_(grads, max_norm: float) -> torch.Tensor:
+    """Multiply `grads` in place by min(1, max_norm / (norm + 1e-6)), norm = their global 2-norm, which is returned (on the GPU, as it was
+    before). Nothing is written where the factor is 1."""
+    if not max_norm >= 0.0:
+        _refuse(f"max_norm {max_norm} >= 0 is wanted")
+    for i, g in enumerate(grads):
+        if g is not None and not g.is_sparse and not _dense(g) and any(st == 0 and k > 1 for st, k in zip(g.stride(), g.shape)):
+            _refuse(f"grads[{i}] is a broadcast view: several elements share a place and cannot be scaled in place")
+    return _clip_call([g for g in grads if g is not None], float(max_norm), None)
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """`clip_grads_` on the gradients of `parameters` (torch.nn.utils.clip_grad_norm_ for the 2-norm)."""
+    if float(norm_type) != 2.0:
+        _refuse(f"norm_type {norm_type}: the 2-norm alone is supported")
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return clip_grads_([p.grad for p in parameters], max_norm)
+
+
+def _state8_call(state: AdamState8, exp_avgs, exp_avg_sqs, write: int) -> None:
+    n = len(exp_avgs)
+    _check_lengths(n, exp_avg_sqs=exp_avg_sqs, exp_avg=state.exp_avg, exp_avg_scale=state.exp_avg_scale, root=state.root, root_scale=state.root_scale)
+    if n == 0:
+        return
+    device = exp_avgs[0].device
+    _check_list("exp_avgs", exp_avgs, torch.float32, device)
+    _check_list("exp_avg_sqs", exp_avg_sqs, torch.float32, device, exp_avgs)
+    _check_list("exp_avg", state.exp_avg, _F8, device, exp_avgs)
+    _check_list("root", state.root, _F8, device, exp_avgs)
+    numel = [t.numel() for t in exp_avgs]
+    _check_scales("exp_avg_scale", state.exp_avg_scale, numel, device)
+    _check_scales("root_scale", state.root_scale, numel, device)
+    _check_distinct("what is written", [*state.exp_avg, *state.root] if write else [*exp_avgs, *exp_avg_sqs])
+    words = _words(n, _ptrs(exp_avgs), _ptrs(exp_avg_sqs), _ptrs(state.exp_avg), _ptrs(state.root), _ptrs(state.exp_avg_scale), _ptrs(state.root_scale),
+                   numel, None, [(L.F32 << 32) | (8 << 48)] * n)
+    _run(device, "nndet_adam_state8", words, n, write)
+
+
+def write_adam_state8(state: AdamState8, exp_avgs, exp_avg_sqs) -> None:
+    """Round fp32 moments into `state`, in place: the first moments and the roots of the second to the nearest code (a root that is not 0
+    to a code that is not 0)."""
+    _state8_call(state, exp_avgs, exp_avg_sqs, 1)
+
+
+def read_adam_state8(state: AdamState8, exp_avgs, exp_avg_sqs) -> None:
+    """The moments that `state` stands for into fp32 tensors, in place."""
+    _state8_call(state, exp_avgs, exp_avg_sqs, 0)
+
+
+class AdamW:
+    """AdamW on the operators above, with the interface of `SGDNesterov`: one call of the library a step for all parameters that share
+    (lr, betas, eps), whatever their weight decays and types.
+
+    param_groups: dicts with "params" and optionally "lr", "betas", "eps", "weight_decay"; or the parameters themselves.
+    state_bits: 32, or 8 (2 bytes an element for both moments instead of 8); a parameter of fewer than `min_8bit_numel` elements keeps 32
+    bits: it would not save anything, and norms and biases have few elements that share a block's scale.
+    max_norm: clip by the global gradient norm within the step (the gradients themselves are not written); `grad_norm` holds the norm of
+    the last step, on the GPU.
+    lr: a number, or one fp32 value on the GPU, which a captured step reads. A step can be captured once every parameter has a state, i.e.
+    after a first step outside of the capture."""
+
+    _step_supports_amp_scaling = True                # torch.amp.GradScaler hands grad_scale / found_inf over as device tensors
+
+    def __init__(self, param_groups, lr: Rate = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
+                 min_8bit_numel: int = 4096, max_norm: Optional[float] = None):
+        if state_bits not in (32, 8):
+            _refuse(f"state_bits {state_bits}: 32 or 8")
+        if max_norm is not None and not max_norm >= 0.0:
+            _refuse(f"max_norm {max_norm} >= 0 is wanted")
+        groups = list(param_groups)
+        if groups and not isinstance(groups[0], dict):
+            groups = [{"params": groups}]
+        self.defaults = {"lr": float(lr), "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay}
+        self.param_groups = []
+        for g in groups:
+            more = set(g) - {"params", "lr", "betas", "eps", "weight_decay"}
+            if more:
+                _refuse(f"unknown entries {sorted(more)} of a parameter group")
+            ps = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
+            self.param_groups.append({"params": [p for p in ps if p.requires_grad], "lr": g.get("lr", lr), "betas": tuple(g.get("betas", betas)),
+                                      "eps": g.get("eps", eps), "weight_decay": float(g.get("weight_decay", weight_decay))})
+        flat = [p for g in self.param_groups for p in g["params"]]
+        if len(set(map(id, flat))) != len(flat):
+            _refuse("a parameter appears twice")
+        _kinds(flat)
+        self.state_bits, self.min_8bit_numel, self.max_norm = state_bits, int(min_8bit_numel), max_norm
+        self.grad_norm: Optional[torch.Tensor] = None
+        self._slot = {p: i for i, p in enumerate(flat)}
+        self._state = {}                             # parameter -> {name: tensor}
+        self._steps = {}                             # device -> int32 counts, one for every parameter
+        self._fixed = {}                             # parameter -> addresses of its state, number of elements, last word of its struct
+
+    def _bits(self, p) -> int:
+        return 8 if self.state_bits == 8 and p.numel() >= self.min_8bit_numel else 32
+
+    def _counts(self, device) -> torch.Tensor:
+        if device not in self._steps:
+            self._steps[device] = torch.zeros((len(self._slot),), dtype=torch.int32, device=device)
+        return self._steps[device]
+
+    def _init_state(self, p) -> None:
+        if not _dense(p):
+            _refuse(f"a parameter with strides {p.stride()} is not dense in memory")
+        if p.device.type != "cuda":
+            _refuse(f"a parameter on {p.device}: nndetection_amd kernels need tensors on the GPU (no CPU path)")
+        if torch.cuda.is_current_stream_capturing():
+            _refuse("a parameter has no state yet: take a step outside of the capture first")
+        if self._bits(p) == 8:
+            self._set_state(p, dict(zip(AdamState8._fields, (x[0] for x in AdamState8.zeros([p])))))
+        else:
+            self._set_state(p, {"exp_avg": torch.zeros_like(p, dtype=torch.float32), "exp_avg_sq": torch.zeros_like(p, dtype=torch.float32)})
+
+    def _set_state(self, p, st: dict) -> None:
+        bits = 8 if "root" in st else 32
+        at = [st[k].data_ptr() if k in st else 0 for k in (("exp_avg", "root", "exp_avg_scale", "root_scale") if bits == 8 else ("exp_avg", "exp_avg_sq", "", ""))]
+        self._state[p] = st
+        self._fixed[p] = (*at, p.numel(), self._slot[p] | _KIND[p.dtype] | (bits << 48), p.stride(), p.device)
+
+    @torch.no_grad()
+    def step(self) -> None:
+        scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        calls = {}
+        for g in self.param_groups:
+            wd = _double_bits(float(g["weight_decay"]))
+            key = (id(g["lr"]) if isinstance(g["lr"], torch.Tensor) else g["lr"], *g["betas"], g["eps"])
+            for p in g["params"]:
+                gr = p.grad
+                if gr is None:
+                    continue
+                fixed = self._fixed.get(p)
+                if fixed is None:
+                    self._init_state(p)
+                    fixed = self._fixed[p]
+                m, v, ms, rs, numel, tail, stride, device = fixed
+                if p.device != device or p.numel() != numel or p.stride() != stride:
+                    _refuse(f"a parameter of shape {tuple(p.shape)} on {p.device} was moved or changed its size after its state was made")
+                if gr.stride() != stride or gr.is_sparse:
+                    gr = _grads_like([p], [gr])[0]
+                c = calls.get((device, key))
+                if c is None:
+                    c = calls[(device, key)] = ([], [], [], g)
+                c[0].extend((p.data_ptr(), gr.data_ptr(), m, v, ms, rs, numel, wd, tail))
+                c[1].append(p)
+                c[2].append(gr)
+        if not calls:
+            return
+        on = lambda t, device: None if t is None else t.to(device)  # noqa: E731
+        total = None
+        if self.max_norm is not None and len(calls) > 1:     # a norm over all of them first
+            per = {}
+            for (device, _), c in calls.items():
+                per.setdefault(device, []).extend(c[2])
+            norms = [grad_norm(gs, on(scale, device)) for device, gs in per.items()]
+            total = norms[0] if len(norms) == 1 else torch.stack([x.to(norms[0].device, torch.float64) for x in norms]).square().sum().sqrt().float()
+        for (device, _), (words, ps, _, g) in calls.items():
+            counts = self._counts(device)
+            a, self.grad_norm = _hyper(g["lr"], g["betas"], g["eps"], self.max_norm, on(total, device), on(scale, device), on(found, device),
+                                       counts, device)
+            _run(device, "nndet_adamw_step", array.array("q", words), len(ps), L.C.byref(a))
+            _written(ps)
+
+    # ---- checkpointing, laid out like torch.optim.AdamW.state_dict(). Parameters with 8-bit moments hold those of `AdamState8` in place of
+    # "exp_avg_sq" (resuming from them is exact); bits=32 writes them as fp32 moments, which torch.optim.AdamW loads. load_state_dict takes
+    # either kind, its own or torch's, whatever state_bits is here.
+    def state_dict(self, bits: Optional[int] = None) -> dict:
+        if bits not in (None, 32):
+            _refuse(f"state_dict(bits={bits}): 32, or None for the moments as they are")
+        state, groups, idx = {}, [], 0
+        for g in self.param_groups:
+            ids = []
+            for p in g["params"]:
+                if p in self._state:
+                    st = dict(self._state[p])
+                    if bits == 32 and "root" in st:
+                        full = torch.empty_like(p, dtype=torch.float32), torch.empty_like(p, dtype=torch.float32)
+                        read_adam_state8(AdamState8(*([st[k]] for k in AdamState8._fields)), [full[0]], [full[1]])
+                        st = dict(zip(("exp_avg", "exp_avg_sq"), full))
+                    state[idx] = {"step": self._counts(p.device)[self._slot[p]].float(), **st}
+                ids.append(idx); idx += 1
+            groups.append({**{k: v for k, v in g.items() if k != "params"}, "amsgrad": False, "maximize": False, "foreach": None, "capturable": False,
+                           "differentiable": False, "fused": None, "decoupled_weight_decay": True, "params": ids})
+        return {"state": state, "param_groups": groups}
+
+    def load_state_dict(self, sd: dict) -> None:
+        groups = sd["param_groups"]
+        if len(groups) != len(self.param_groups) or any(len(a["params"]) != len(b["params"]) for a, b in zip(groups, self.param_groups)):
+            raise ValueError("loaded state dict has different parameter groups")
+        if any(g.get("amsgrad") or g.get("maximize") for g in groups):
+            raise ValueError("amsgrad and maximize are not supported")
+        flat = [p for g in self.param_groups for p in g["params"]]
+        like = lambda t, p, dtype: torch.empty_like(p, dtype=dtype).copy_(t.detach())  # noqa: E731
+        self._state, self._fixed, self._steps = {}, {}, {}
+        for k, st in sd["state"].items():
+            p = flat[int(k)]
+            if tuple(st["exp_avg"].shape) != tuple(p.shape):
+                raise ValueError(f"loaded moments of parameter {k} have shape {tuple(st['exp_avg'].shape)}, the parameter {tuple(p.shape)}")
+            if "root" in st:
+                new = {"exp_avg": like(st["exp_avg"].view(torch.uint8), p, torch.uint8).view(_F8), "exp_avg_scale": st["exp_avg_scale"].detach().to(p.device).clone(),
+                       "root": like(st["root"].view(torch.uint8), p, torch.uint8).view(_F8), "root_scale": st["root_scale"].detach().to(p.device).clone()}
+            else:
+                new = {"exp_avg": like(st["exp_avg"], p, torch.float32), "exp_avg_sq": like(st["exp_avg_sq"], p, torch.float32)}
+            have = 8 if "root" in new else 32
+            if have != self._bits(p):
+                st8 = AdamState8.zeros([p]) if have == 32 else AdamState8(*([new[f]] for f in AdamState8._fields))
+                full = [new["exp_avg"], new["exp_avg_sq"]] if have == 32 else [torch.empty_like(p, dtype=torch.float32) for _ in range(2)]
+                (write_adam_state8 if have == 32 else read_adam_state8)(st8, full[:1], full[1:])
+                new = dict(zip(AdamState8._fields, (x[0] for x in st8))) if have == 32 else dict(zip(("exp_avg", "exp_avg_sq"), full))
+            self._set_state(p, new)
+            self._counts(p.device)[self._slot[p]] = int(st["step"])
+        for g, src in zip(self.param_groups, groups):
+            if isinstance(g["lr"], torch.Tensor):
+                g["lr"].fill_(float(src["lr"]))
+            else:
+                g["lr"] = float(src["lr"])
+            g["betas"], g["eps"], g["weight_decay"] = tuple(src["betas"]), float(src["eps"]), float(src["weight_decay"])
+
+    zero_grad = SGDNesterov.zero_grad
+
+
 class LinearWarmupPolyLR:
     """lr(k) with k = number of scheduler steps + 1, exactly the reference's `_step_count` arithmetic."""
 
-    def __init__(self, optimizer: SGDNesterov, warm_iterations: int, warm_lr: float, poly_gamma: float, num_iterations: int):
+    def __init__(self, optimizer: Union[SGDNesterov, AdamW], warm_iterations: int, warm_lr: float, poly_gamma: float, num_iterations: int):
         self.opt, self.warm, self.warm_lr, self.gamma, self.total = optimizer, warm_iterations, warm_lr, poly_gamma, num_iterations
         self.base_lr = optimizer.defaults["lr"]
         self._step_count = 0
@@ -154,9 +651,14 @@ class LinearWarmupPolyLR:
 
     def step(self):
         self._step_count += 1
-        lr = self.get_lr()
+        self._set(self.get_lr())
+
+    def _set(self, lr: float) -> None:
         for g in self.opt.param_groups:
-            g["lr"] = lr
+            if isinstance(g["lr"], torch.Tensor):                     # a rate on the device (AdamW): what a captured step reads
+                g["lr"].fill_(lr)
+            else:
+                g["lr"] = lr
 
     def state_dict(self) -> dict:
         """`_step_count` / `last_epoch` as torch's _LRScheduler keeps them (last_epoch = _step_count - 1)."""
@@ -164,6 +666,4 @@ class LinearWarmupPolyLR:
 
     def load_state_dict(self, sd: dict) -> None:
         self._step_count = int(sd["_step_count"])
-        lr = self.get_lr()
-        for g in self.opt.param_groups:
-            g["lr"] = lr
+        self._set(self.get_lr())

@@ -98,16 +98,29 @@ def get_params_no_wd_on_norm(model: nn.Module, weight_decay: float) -> List[dict
 def configure_optimizer(model: nn.Module, trainer_cfg: dict = None, lean: bool = True):
     """SGD(nesterov) + linear warm-up -> poly decay, stepped per iteration (retinaunet/base.py:300-336).
     lean=True: the foreach-based implementation of nndetection_amd/optim.py (same arithmetic, far less host time);
-    lean=False: torch.optim.SGD + LambdaLR."""
+    lean=False: torch.optim.SGD + LambdaLR.
+    trainer_cfg["optimizer"] = "adamw" / "adamw8" (default "sgd"): AdamW on the same groups and schedule, with moments in 32 / 8 bits
+    (lean=False: torch.optim.AdamW); "adamw_betas", "adamw_eps" and "max_norm" (clipping within the step, lean only) go with it."""
     cfg = dict(TRAINER_CFG_V001 if trainer_cfg is None else trainer_cfg)
     groups = get_params_no_wd_on_norm(model, cfg["weight_decay"])
     total = cfg["max_num_epochs"] * cfg["num_train_batches_per_epoch"]
     warm, warm_lr, lr0, gamma = cfg["warm_iterations"], cfg["warm_lr"], cfg["initial_lr"], cfg["poly_gamma"]
+    kind = cfg.get("optimizer", "sgd")
+    if kind not in ("sgd", "adamw", "adamw8"):
+        raise ValueError(f"trainer_cfg['optimizer'] = {kind!r}: 'sgd', 'adamw' or 'adamw8'")
+    if kind != "sgd" and lean:
+        from .optim import AdamW, LinearWarmupPolyLR
+        opt = AdamW(groups, lr0, betas=cfg.get("adamw_betas", (0.9, 0.999)), eps=cfg.get("adamw_eps", 1e-8),
+                    state_bits=8 if kind == "adamw8" else 32, max_norm=cfg.get("max_norm"))
+        return opt, LinearWarmupPolyLR(opt, warm, warm_lr, gamma, total)
     if lean:
         from .optim import SGDNesterov, LinearWarmupPolyLR
         opt = SGDNesterov(groups, lr0, momentum=cfg["sgd_momentum"], nesterov=cfg["sgd_nesterov"])
         return opt, LinearWarmupPolyLR(opt, warm, warm_lr, gamma, total)
-    opt = torch.optim.SGD(groups, lr0, weight_decay=cfg["weight_decay"], momentum=cfg["sgd_momentum"], nesterov=cfg["sgd_nesterov"])
+    if kind != "sgd":
+        opt = torch.optim.AdamW(groups, lr0, betas=cfg.get("adamw_betas", (0.9, 0.999)), eps=cfg.get("adamw_eps", 1e-8))
+    else:
+        opt = torch.optim.SGD(groups, lr0, weight_decay=cfg["weight_decay"], momentum=cfg["sgd_momentum"], nesterov=cfg["sgd_nesterov"])
 
     def factor(it: int) -> float:                 # it = number of scheduler steps so far; the reference uses k = it + 1
         k = it + 1
