@@ -175,6 +175,22 @@ SIGNATURES = {
 }
 
 _lib = None
+_host_lists = None
+
+
+def host_lists():
+    """The module csrc/nndet_host.so (built with the library): lists of tensors to the structs of an optimiser call."""
+    global _host_lists
+    if _host_lists is None:
+        import importlib.machinery
+        import importlib.util
+        path = os.path.join(_HERE, "csrc", "nndet_host.so")
+        if not os.path.isfile(path):
+            raise NndetError(f"{path} not found: build it with nndetection_amd/csrc/build.sh")
+        spec = importlib.util.spec_from_loader("nndet_host", importlib.machinery.ExtensionFileLoader("nndet_host", path))
+        _host_lists = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_host_lists)
+    return _host_lists
 
 
 def load():

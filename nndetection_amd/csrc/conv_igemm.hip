@@ -1142,7 +1142,10 @@ __global__ __launch_bounds__(256, 1) void k_ig3r(const Ig3rArgs A) {
             const v2u_t r = __builtin_amdgcn_permlane16_swap(epk[0][h], epk[1][h], false, false);
             est[h] = r[0]; est[2 + h] = r[1];
         }
-        else if (m == 14) __builtin_amdgcn_raw_buffer_store_b128(est, yrs, vlane, soff, 0);
+        else if (m == 14) {
+            __builtin_amdgcn_raw_buffer_store_b128(est, yrs, vlane, soff, 0);
+            asm volatile("s_nop 0");                                    // (the next micro-ops may reuse est's registers: store-data hazard, see the last tile)
+        }
         else if (m < 23) { const int i = (m - 15) >> 2, r = (m - 15) & 3; ev[i][r] = (r & 1) ? H16<T>::hi(epk[i][r >> 1]) : H16<T>::lo(epk[i][r >> 1]); }
         else if (m < 31) { const int i = (m - 23) >> 2, r = (m - 23) & 3; ssum[i][r] += ev[i][r]; }
         else { const int i = (m - 31) >> 2, r = (m - 31) & 3; ssq[i][r] = fmaf(ev[i][r], ev[i][r], ssq[i][r]); }

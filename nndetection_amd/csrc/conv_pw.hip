@@ -204,7 +204,10 @@ __global__ __launch_bounds__(256) void k_pw(const PwArgs A) {
                             }
                             const pw_v2u s0 = __builtin_amdgcn_permlane16_swap(pk[0][0], pk[1][0], false, false);
                             const pw_v2u s1 = __builtin_amdgcn_permlane16_swap(pk[0][1], pk[1][1], false, false);
-                            if (pv) *reinterpret_cast<u32x4*>(yb + o * A.Cy + row0 + i * 16 + (q >> 1) * 8 + (q & 1) * 16) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                            if (pv) {
+                                *reinterpret_cast<u32x4*>(yb + o * A.Cy + row0 + i * 16 + (q >> 1) * 8 + (q & 1) * 16) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                                asm volatile("s_nop 0");     // (the store's data registers may be the next ones written: store-data hazard)
+                            }
                         }
                     } else if (pv) {
                         T* yo = yb + o * A.Cy + row0 + q * 4;
@@ -267,7 +270,10 @@ __global__ __launch_bounds__(256) void k_pw(const PwArgs A) {
                     for (int i = 0; i < MT; i += 2) {
                         const pw_v2u s0 = __builtin_amdgcn_permlane16_swap(H16<T>::pack2(acc[i][0], acc[i][1]), H16<T>::pack2(acc[i + 1][0], acc[i + 1][1]), false, false);
                         const pw_v2u s1 = __builtin_amdgcn_permlane16_swap(H16<T>::pack2(acc[i][2], acc[i][3]), H16<T>::pack2(acc[i + 1][2], acc[i + 1][3]), false, false);
-                        if (ok) *reinterpret_cast<u32x4*>(yb + p * A.Cy + row0 + i * 16 + (q >> 1) * 8 + (q & 1) * 16) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                        if (ok) {
+                                *reinterpret_cast<u32x4*>(yb + p * A.Cy + row0 + i * 16 + (q >> 1) * 8 + (q & 1) * 16) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                                asm volatile("s_nop 0");     // (the store's data registers may be the next ones written: store-data hazard)
+                            }
                     }
                 } else if (ok) {
                     T* yo = yb + p * A.Cy + row0 + q * 4;

@@ -1,0 +1,181 @@
+// Fast path of the optimiser's host side: the tensors of a call to the NndetOptTensor structs of include/nndet_amd.h.
+//
+// The checks that nndetection_amd/optim.py makes of every tensor (device, type, shape, density, distinct addresses) cost it about 2 us a
+// tensor, more than the GPU needs for the step of a network of 92 tensors. pack() makes the same checks here, a few ns each. It knows the
+// ordinary case alone -- everything dense on one GPU, in one memory order -- and answers None for anything else: then optim.py looks itself, copies
+// what lies in another order, and words the refusal.
+#include <torch/csrc/autograd/python_variable.h>
+#include <ATen/core/TensorBody.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "../../include/nndet_amd.h"
+
+namespace {
+
+struct List {                                        // a list or tuple, or nothing
+    PyObject* seq = nullptr;
+    Py_ssize_t n = 0;
+    bool take(PyObject* o) {
+        if (o == Py_None) return true;
+        if (!PyList_CheckExact(o) && !PyTuple_Check(o)) return false;
+        seq = o;
+        n = PySequence_Fast_GET_SIZE(o);
+        return true;
+    }
+    PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(seq, i); }
+};
+
+// `o` as a plain dense GPU tensor on `device`, or nullptr
+const c10::TensorImpl* plain(const at::TensorBase& t, c10::DeviceIndex device) {
+    if (!t.defined()) return nullptr;
+    const c10::TensorImpl* x = t.unsafeGetTensorImpl();
+    if (x->layout() != c10::kStrided || x->is_python_dispatch() || x->device() != c10::Device(c10::kCUDA, device)) return nullptr;
+    if (!x->is_non_overlapping_and_dense() || (x->numel() && !x->data())) return nullptr;
+    return x;
+}
+const c10::TensorImpl* plain(PyObject* o, c10::DeviceIndex device) {
+    return THPVariable_Check(o) ? plain(THPVariable_Unpack(o), device) : nullptr;
+}
+
+// of one shape, and in one memory order
+bool same(const c10::TensorImpl* a, const c10::TensorImpl* b) {
+    return a->sizes().equals(b->sizes()) && ((a->is_contiguous() && b->is_contiguous()) || a->strides().equals(b->strides()));
+}
+
+int type_of(const c10::TensorImpl* x) {
+    switch (c10::typeMetaToScalarType(x->dtype())) {
+        case c10::ScalarType::Float: return NNDET_F32;
+        case c10::ScalarType::BFloat16: return NNDET_BF16;
+        case c10::ScalarType::Half: return NNDET_F16;
+        default: return -1;
+    }
+}
+bool is(const c10::TensorImpl* x, c10::ScalarType t) { return c10::typeMetaToScalarType(x->dtype()) == t; }
+
+// pack(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, root_scales, weight_decay, bits, device,
+//      both) -> (structs, n) or None
+//   params None: grads alone. grads None: params[i].grad. A gradient that is None leaves its tensor out (slot = place in the list).
+//   exp_avgs None: no moments. bits: 32, 8, or 0 for either, by the type of exp_avgs[i]. weight_decay: a number or a list.
+//   both: grads are written too.
+PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 10) {
+        PyErr_SetString(PyExc_TypeError, "pack() takes 10 arguments");
+        return nullptr;
+    }
+    try {
+        List p, g, m, v, ms, rs, wd;
+        const bool listed = PyList_CheckExact(args[6]) || PyTuple_Check(args[6]);
+        if (!p.take(args[0]) || !g.take(args[1]) || !m.take(args[2]) || !v.take(args[3]) || !ms.take(args[4]) || !rs.take(args[5]) || (listed && !wd.take(args[6])))
+            Py_RETURN_NONE;
+        const double one_wd = listed ? 0.0 : PyFloat_AsDouble(args[6]);
+        const long bits = PyLong_AsLong(args[7]), device = PyLong_AsLong(args[8]), both = PyLong_AsLong(args[9]);
+        if (PyErr_Occurred()) return nullptr;
+        const Py_ssize_t n = p.seq ? p.n : g.n;
+        if ((!p.seq && !g.seq) || n >= (1 << 24) || (g.seq && g.n != n) || (m.seq && (!v.seq || m.n != n || v.n != n)) || (listed && wd.n != n)) Py_RETURN_NONE;
+        if (ms.seq && (!rs.seq || ms.n != n || rs.n != n)) Py_RETURN_NONE;
+        PyObject* out = PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(NndetOptTensor));
+        if (!out) return nullptr;
+        NndetOptTensor* t = reinterpret_cast<NndetOptTensor*>(PyBytes_AS_STRING(out));
+        std::vector<void*> at;
+        at.reserve(4 * n);
+        Py_ssize_t k = 0;
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            const c10::TensorImpl *px = nullptr, *gx = nullptr;
+            if (g.seq && g[i] == Py_None) continue;
+            if (p.seq) {
+                px = plain(p[i], device);
+                if (!px) goto other;
+            }
+            if (g.seq) {
+                gx = plain(g[i], device);
+            } else {
+                const at::Tensor& grad = THPVariable_Unpack(p[i]).grad();
+                if (!grad.defined()) continue;
+                gx = plain(grad, device);
+            }
+            if (!gx) goto other;
+            NndetOptTensor& e = t[k];
+            memset(&e, 0, sizeof(e));
+            const c10::TensorImpl* x = px ? px : gx;
+            const int type = type_of(x);
+            if (type < 0 || (px && (px->dtype() != gx->dtype() || !same(px, gx)))) goto other;
+            e.param = px ? const_cast<void*>(px->data()) : nullptr;
+            e.grad = const_cast<void*>(gx->data());
+            e.numel = x->numel();
+            e.slot = (int32_t)i;
+            e.dtype = (int16_t)type;
+            e.state_bits = 32;
+            if (listed) {
+                e.weight_decay = PyFloat_AsDouble(wd[i]);
+                if (e.weight_decay == -1.0 && PyErr_Occurred()) { PyErr_Clear(); goto other; }
+            } else {
+                e.weight_decay = one_wd;
+            }
+            if (m.seq) {
+                const c10::TensorImpl *mx = plain(m[i], device), *vx = plain(v[i], device);
+                if (!mx || !vx || !same(mx, x) || !same(vx, x) || mx->dtype() != vx->dtype()) goto other;
+                e.exp_avg = const_cast<void*>(mx->data());
+                e.exp_avg_sq = const_cast<void*>(vx->data());
+                if (is(mx, c10::ScalarType::Float8_e4m3fn) && bits != 32 && ms.seq) {
+                    const c10::TensorImpl *sx = plain(ms[i], device), *rx = plain(rs[i], device);
+                    const int64_t blocks = (e.numel + 255) / 256;
+                    if (!sx || !rx || !is(sx, c10::ScalarType::Float) || !is(rx, c10::ScalarType::Float) || sx->numel() != blocks || rx->numel() != blocks) goto other;
+                    e.exp_avg_scale = (float*)const_cast<void*>(sx->data());
+                    e.root_scale = (float*)const_cast<void*>(rx->data());
+                    e.state_bits = 8;
+                } else if (!is(mx, c10::ScalarType::Float) || bits == 8) {
+                    goto other;
+                }
+            }
+            if (e.numel) {                           // what a call writes: no address twice
+                at.push_back(e.param ? e.param : e.grad);
+                if (px && both) at.push_back(e.grad);
+                if (m.seq) { at.push_back(e.exp_avg); at.push_back(e.exp_avg_sq); }
+            }
+            ++k;
+        }
+        std::sort(at.begin(), at.end());
+        if (std::adjacent_find(at.begin(), at.end()) != at.end()) goto other;
+        if (k != n && _PyBytes_Resize(&out, k * (Py_ssize_t)sizeof(NndetOptTensor)) < 0) return nullptr;
+        return Py_BuildValue("Nn", out, k);
+    other:
+        Py_DECREF(out);
+        Py_RETURN_NONE;
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// written(tensors, grads): advance the version counters of the tensors (of those with a gradient, unless grads is None)
+PyObject* written(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    List t, g;
+    if (nargs != 2 || !t.take(args[0]) || !g.take(args[1]) || (g.seq && g.n != t.n)) {
+        PyErr_SetString(PyExc_TypeError, "written(tensors, grads) takes two lists of one length");
+        return nullptr;
+    }
+    try {
+        for (Py_ssize_t i = 0; i < t.n; ++i) {
+            if ((g.seq && g[i] == Py_None) || !THPVariable_Check(t[i])) continue;
+            const at::Tensor& x = THPVariable_Unpack(t[i]);
+            if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+        }
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+    Py_RETURN_NONE;
+}
+
+PyMethodDef methods[] = {
+    {"pack", (PyCFunction)(void (*)(void))pack, METH_FASTCALL, nullptr},
+    {"written", (PyCFunction)(void (*)(void))written, METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr},
+};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "nndet_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_nndet_host() { return PyModule_Create(&module); }

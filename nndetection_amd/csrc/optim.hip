@@ -2,7 +2,7 @@
 // conversion between fp32 and 8-bit moments.
 //
 // A call takes n tensors of any sizes. k_opt_table copies their addresses out of the kernel arguments into a table in the workspace (64 B
-// a tensor, OPT_ARGS of them a launch, so that every later kernel is ONE launch whatever n is), advances the step counts and works out what
+// a tensor, up to 99 of them a launch, so that every later kernel is ONE launch whatever n is), advances the step counts and works out what
 // is the same for a whole tensor. Then one launch per storage kind walks over tiles of 1024 consecutive elements of a tensor; no tile spans
 // two tensors. A wave owns 256 consecutive elements of its tile, which is also the block that shares a scale of the 8-bit moments: the
 // block maximum never leaves the wave.
@@ -20,34 +20,60 @@
 // from the code below: the expected value of the stored r is r. The 16 random bits an element come from its index in the tensor and
 // t alone (opt_mix), so a step is reproducible. An r that is not zero is not stored as zero: m / (0 + eps) would be a step of any size.
 #include "common.h"
+#include <math.h>
+#include <stddef.h>
 #include <string.h>
 
 static constexpr int OPT_WG = 256;               // threads of a workgroup: 4 waves
 static constexpr int OPT_BLOCK = 256;            // elements of a wave's block = elements that share a scale
-static constexpr int OPT_TILE = 1024;            // elements of a workgroup's tile
-static constexpr int OPT_ARGS = 62;              // tensors per k_opt_table launch: 62 * 64 B + 88 B of scalars stay below 4 KB of arguments
+#ifndef OPT_NB
+#define OPT_NB 2
+#endif
+#ifndef OPT_U
+#define OPT_U 2
+#endif
+#ifndef OPT_G
+#define OPT_G 1000000
+#endif
+#ifndef OPT_NT
+#define OPT_NT 3
+#endif
+#ifndef OPT_CLIP_NB
+#define OPT_CLIP_NB 4
+#endif
 static constexpr int OPT_PARTIALS = 1024;        // workgroups (and fp64 partial sums) of the norm per storage type
-static constexpr int OPT_GRID = 2048;            // workgroups of a walk over the tiles: 8 for each of the 256 CUs
+static constexpr int OPT_GRID = OPT_G;            // workgroups of a walk over the tiles: 8 for each of the 256 CUs
 
 struct OptEntry {                                // one tensor in the workspace's table
     void* p; const void* g; void* m; void* v; float* ms; float* rs;
     int64_t numel;
-    uint32_t tile0, pad;                         // first tile within its launch
+    uint64_t pad;
 };
+static_assert(sizeof(OptEntry) == 64, "four 16-byte stores");
 struct OptCoef { float size, unbias, decay; uint32_t t; };
 struct OptHead { float factor; int32_t skip; int32_t pad[14]; };
 
-struct OptArg { void* p; const void* g; void* m; void* v; float* ms; float* rs; uint64_t numel_slot; float wd; uint32_t tile0; };
-struct OptTableArgs {
-    OptHead* head; OptEntry* entry; OptCoef* coef; int32_t* steps;
+// A tensor in the kernel arguments: its PTRS addresses (48 bits each; 4: param, grad, moments, 6: and the scales), numel below 2^40, slot.
+template <int PTRS> struct OptArg { uint32_t lo[PTRS]; uint16_t hi[PTRS]; uint32_t numel_lo, numel_hi_slot; float wd; uint32_t tile0; };
+template <int PTRS> struct OptTableArgs {
+    static constexpr int MOST = PTRS == 4 ? 99 : 76;     // tensors a launch: what 4 KB of kernel arguments hold
+    OptHead* head; OptEntry* entry; OptCoef* coef; uint32_t* tile0; int32_t* steps;
     const float* lr_ptr; const float* found_inf; const float* grad_scale;
-    double lr, b1, b2;
-    int32_t n, first;                            // entries of this launch; first: it also writes the head
-    OptArg a[OPT_ARGS];
+    double lr, log2_b1, log2_b2;
+    int32_t n, first;                                    // tensors of this launch; first: it also writes the head
+    OptArg<PTRS> a[MOST];
 };
-static_assert(sizeof(OptTableArgs) <= 4096, "kernel arguments are limited to 4 KB");
+static_assert(sizeof(OptTableArgs<4>) <= 4096 && sizeof(OptTableArgs<6>) <= 4096, "kernel arguments are limited to 4 KB");
 
-__global__ __launch_bounds__(64) void k_opt_table(const OptTableArgs A) {
+// After 16-byte stores, with all arithmetic before them (a sched_barrier): nothing may overwrite a store's data registers in its next slots
+// (tools/scan_store_hazard.py).
+__device__ __forceinline__ void opt_stored() {
+    asm volatile("s_nop 0");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int PTRS>
+__global__ __launch_bounds__(128) void k_opt_table(const OptTableArgs<PTRS> A) {
     const int i = threadIdx.x;
     const bool skip = A.found_inf && *A.found_inf != 0.0f;
     if (A.first && i == 0) {
@@ -55,20 +81,31 @@ __global__ __launch_bounds__(64) void k_opt_table(const OptTableArgs A) {
         A.head->factor = A.grad_scale ? (float)(1.0 / (double)*A.grad_scale) : 1.0f;   // (the norm's kernel writes it again)
     }
     if (i >= A.n) return;
-    const OptArg& a = A.a[i];
-    OptEntry e = {a.p, a.g, a.m, a.v, a.ms, a.rs, (int64_t)(a.numel_slot & ((1ull << 40) - 1)), a.tile0, 0};
-    A.entry[i] = e;
+    const OptArg<PTRS>& a = A.a[i];
+    uint64_t at[6] = {0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < PTRS; ++k) at[k] = a.lo[k] | (uint64_t)a.hi[k] << 32;
+    const uint64_t w[8] = {at[0], at[1], at[2], at[3], at[4], at[5], a.numel_lo | (uint64_t)(a.numel_hi_slot & 0xffu) << 32, 0};
+    u32x4 v[4];
+    __builtin_memcpy(v, w, sizeof(v));
+    u32x4* to = (u32x4*)(A.entry + i);
+    A.tile0[i] = a.tile0;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) to[k] = v[k];
+    opt_stored();
     if (!A.steps) return;
-    const uint32_t slot = (uint32_t)(a.numel_slot >> 40);
+    const uint32_t slot = a.numel_hi_slot >> 8;
     const int32_t t = A.steps[slot] + 1;
     if (!skip) A.steps[slot] = t;
     const double lr = A.lr_ptr ? (double)*A.lr_ptr : A.lr;
     OptCoef c;
-    c.size = (float)(lr / (1.0 - pow(A.b1, (double)t)));
-    c.unbias = (float)(1.0 / sqrt(1.0 - pow(A.b2, (double)t)));
+    c.size = (float)(lr / (1.0 - exp2((double)t * A.log2_b1)));
+    c.unbias = (float)(1.0 / sqrt(1.0 - exp2((double)t * A.log2_b2)));
     c.decay = (float)(1.0 - lr * (double)a.wd);
     c.t = (uint32_t)t;
     A.coef[i] = c;
+    opt_stored();
 }
 
 // The table is written by an earlier kernel and constant in this one: read it through the scalar cache, so that what is uniform for a
@@ -83,39 +120,46 @@ template <typename T> __device__ __forceinline__ T opt_uniform(const T* p) {
     return x;
 }
 
-// index of the tensor whose tiles contain `tile`: the last entry with tile0 <= tile (entries are in order of tile0). One ballot per 64 tensors.
-__device__ __forceinline__ int opt_find(const OptEntry* e, int n, uint32_t tile) {
+// index of the tensor whose tiles contain `tile`: the last one with tile0 <= tile (tile0 does not decrease). 256 tensors a round, one latency.
+__device__ __forceinline__ int opt_find(const uint32_t* tile0, int n, uint32_t tile) {
     const int lane = threadIdx.x & 63;
     int found = 0;
-    for (int b = 0; b < n; b += 64) {
-        const bool le = b + lane < n && e[b + lane].tile0 <= tile;
-        const int c = __popcll(__ballot(le));
+    for (int b = 0; b < n; b += 256) {
+        uint32_t t[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = b + 64 * k + lane < n ? tile0[b + 64 * k + lane] : 0xffffffffu;
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c += __popcll(__ballot(t[k] <= tile));
         found += c;
-        if (c < 64) break;
+        if (c < 256) break;
     }
     return __builtin_amdgcn_readfirstlane(found - 1);
 }
 
 // The walk of a workgroup over the tiles blockIdx.x, blockIdx.x + gridDim.x, ...: at any time the chip works on neighbouring addresses (few
 // pages, few open DRAM rows). The tensor is looked up again only when the walk leaves it.
-struct OptWalk {
-    const OptEntry* e; int n; uint32_t tiles, tile, end;
+template <int NB> struct OptWalk {
+    static constexpr int TILE = NB * 4 * OPT_BLOCK;
+    const OptEntry* e; const uint32_t* tile0; int n; uint32_t tiles, tile, start, end;
     int i;
     OptEntry cur;
-    __device__ OptWalk(const OptEntry* e_, int n_, uint32_t tiles_) : e(e_), n(n_), tiles(tiles_), tile(blockIdx.x), end(0), i(-1) {}
+    __device__ OptWalk(const OptEntry* e_, const uint32_t* t0, int n_, uint32_t tiles_) : e(e_), tile0(t0), n(n_), tiles(tiles_), tile(blockIdx.x), end(0), i(-1) {}
     __device__ __forceinline__ void next() { tile += gridDim.x; }
     __device__ __forceinline__ bool enter() {    // true if the tile is another tensor's than the last one
         if (tile < end) return false;
-        i = opt_find(e, n, tile);
+        i = opt_find(tile0, n, tile);
         cur = opt_uniform(e + i);
-        end = i + 1 < n ? opt_uniform(&e[i + 1].tile0) : tiles;
+        start = opt_uniform(tile0 + i);
+        end = i + 1 < n ? opt_uniform(tile0 + i + 1) : tiles;
         return true;
     }
-    // this wave's block: its first element, and how many of its elements there are (<= 0: none)
-    __device__ __forceinline__ int64_t base() const { return (int64_t)(tile - cur.tile0) * OPT_TILE + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * OPT_BLOCK; }
-    __device__ __forceinline__ int rem() const {
+    // A tile is NB rounds of four blocks, one a wave. First element of this wave's first block (its others follow 4 * OPT_BLOCK apart), and how
+    // many elements of the tensor there are from it on (<= 0: none).
+    __device__ __forceinline__ int64_t base() const { return (int64_t)(tile - start) * TILE + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * OPT_BLOCK; }
+    __device__ __forceinline__ int left() const {
         const int64_t r = cur.numel - base();
-        return r < OPT_BLOCK ? (int)r : OPT_BLOCK;        // (a tile is not empty: r > -OPT_TILE)
+        return r < TILE ? (int)r : TILE;                  // (a tile is not empty: r > -TILE)
     }
     // whether four elements of p (wp) and g (wg) are aligned vectors of T, and m and v are aligned to ms bytes (0: not used)
     template <typename T> __device__ __forceinline__ bool aligned(int wp, int wg, int ms) const {
@@ -136,9 +180,9 @@ template <> struct OptVec4<float> { typedef f32x4 type; };
 template <> struct OptVec4<bf16_t> { typedef bf16_t type __attribute__((ext_vector_type(4))); };
 template <> struct OptVec4<f16_t> { typedef f16_t type __attribute__((ext_vector_type(4))); };
 
-template <bool FULL, typename T> __device__ __forceinline__ void opt_load(OptPtr<T> p, int lane, int rem, float* x) {
+template <bool FULL, bool ONCE = false, typename T> __device__ __forceinline__ void opt_load(OptPtr<T> p, int lane, int rem, float* x) {
     if constexpr (FULL) {
-        const auto v = ((OptPtr<typename OptVec4<T>::type>)p)[lane];
+        const auto v = ONCE && (OPT_NT & 1) ? __builtin_nontemporal_load(((OptPtr<typename OptVec4<T>::type>)p) + lane) : ((OptPtr<typename OptVec4<T>::type>)p)[lane];
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = Elem<T>::ld(v[k]);
     } else {
@@ -146,12 +190,13 @@ template <bool FULL, typename T> __device__ __forceinline__ void opt_load(OptPtr
         for (int k = 0; k < 4; ++k) x[k] = lane + 64 * k < rem ? Elem<T>::ld(p[lane + 64 * k]) : 0.0f;
     }
 }
-template <bool FULL, typename T> __device__ __forceinline__ void opt_store(OptPtr<T> p, int lane, int rem, const float* x) {
+template <bool FULL, bool ONCE = false, typename T> __device__ __forceinline__ void opt_store(OptPtr<T> p, int lane, int rem, const float* x) {
     if constexpr (FULL) {
         typename OptVec4<T>::type v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = Elem<T>::st(x[k]);
-        ((OptPtr<typename OptVec4<T>::type>)p)[lane] = v;
+        if (ONCE && (OPT_NT & 2)) __builtin_nontemporal_store(v, ((OptPtr<typename OptVec4<T>::type>)p) + lane);
+        else ((OptPtr<typename OptVec4<T>::type>)p)[lane] = v;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -159,14 +204,14 @@ template <bool FULL, typename T> __device__ __forceinline__ void opt_store(OptPt
     }
 }
 template <bool FULL> __device__ __forceinline__ uint32_t opt_load_codes(OptPtr<uint8_t> p, int lane, int rem) {
-    if constexpr (FULL) return ((OptPtr<uint32_t>)p)[lane];
+    if constexpr (FULL) return OPT_NT & 1 ? __builtin_nontemporal_load((OptPtr<uint32_t>)p + lane) : ((OptPtr<uint32_t>)p)[lane];
     uint32_t c = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) c |= (lane + 64 * k < rem ? (uint32_t)p[lane + 64 * k] : 0u) << (8 * k);
     return c;
 }
 template <bool FULL> __device__ __forceinline__ void opt_store_codes(OptPtr<uint8_t> p, int lane, int rem, uint32_t c) {
-    if constexpr (FULL) { ((OptPtr<uint32_t>)p)[lane] = c; return; }
+    if constexpr (FULL) { if (OPT_NT & 2) __builtin_nontemporal_store(c, (OptPtr<uint32_t>)p + lane); else ((OptPtr<uint32_t>)p)[lane] = c; return; }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         if (lane + 64 * k < rem) p[lane + 64 * k] = (uint8_t)(c >> (8 * k));
@@ -230,129 +275,173 @@ template <bool FULL> __device__ __forceinline__ uint32_t opt_encode_root(const f
     return c;
 }
 
+// Runs f over the blocks of the walk's tiles: f(Full<U>, base) on U whole blocks of an aligned tensor (4 * OPT_BLOCK apart), f(Part, base, rem) on
+// one block of rem elements. `enter` is called when the walk comes to another tensor, `aligned` tells whether that may use vectors.
+template <int U> struct OptWhole { static constexpr bool FULL = true; static constexpr int N = U; };
+struct OptPart { static constexpr bool FULL = false; static constexpr int N = 1; };
+template <int NB, int U, typename W, typename E, typename F> __device__ __forceinline__ void opt_blocks(W& w, E enter, F f) {
+    static_assert(NB % U == 0, "whole steps");
+    bool aligned = false;
+    for (; w.tile < w.tiles; w.next()) {
+        if (w.enter()) aligned = enter();
+        int64_t base = w.base();
+        int left = w.left();
+        if (aligned && left >= (NB - 1) * 4 * OPT_BLOCK + OPT_BLOCK) {
+#pragma unroll 1
+            for (int u = 0; u < NB; u += U) f(OptWhole<U>(), base + u * 4 * OPT_BLOCK, OPT_BLOCK);
+            continue;
+        }
+        for (; left > 0; left -= 4 * OPT_BLOCK, base += 4 * OPT_BLOCK) {
+            if (aligned && left >= OPT_BLOCK) f(OptWhole<1>(), base, OPT_BLOCK);
+            else f(OptPart(), base, left < OPT_BLOCK ? left : OPT_BLOCK);
+        }
+    }
+}
+
 struct OptHyper { float b1, omb1, b2, omb2, eps; };
 
-template <typename T, int BITS, bool FULL>
+template <typename T, int BITS, bool FULL, int U>
 __device__ __forceinline__ void adamw_block(const OptEntry& e, int64_t base, int rem, const OptCoef& c, const OptHyper& H, float factor, int lane) {
-    float p[4], g[4], m[4], v[4], r[4];
+    float p[U][4], g[U][4], m[U][4], v[U][4];
+    uint32_t cm[U], cv[U];
+    float sm[U], sr[U];
     const int64_t block = base / OPT_BLOCK;
-    opt_load<FULL>(opt_at<T>(e.g, base), lane, rem, g);
-    if constexpr (BITS == 8) {
-        const uint32_t cm = opt_load_codes<FULL>(opt_at<uint8_t>(e.m, base), lane, rem);
-        const uint32_t cv = opt_load_codes<FULL>(opt_at<uint8_t>(e.v, base), lane, rem);
-        const float sm = *opt_at<float>(e.ms, block), sr = *opt_at<float>(e.rs, block);
-        opt_load<FULL>(opt_at<T>(e.p, base), lane, rem, p);
-        opt_decode(cm, sm, m);
-        opt_decode(cv, sr, v);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = v[k] * v[k];
-    } else {
-        opt_load<FULL>(opt_at<float>(e.m, base), lane, rem, m);
-        opt_load<FULL>(opt_at<float>(e.v, base), lane, rem, v);
-        opt_load<FULL>(opt_at<T>(e.p, base), lane, rem, p);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        g[k] = g[k] * factor;
-        m[k] = m[k] * H.b1 + g[k] * H.omb1;
-        v[k] = v[k] * H.b2 + (g[k] * g[k]) * H.omb2;
-        r[k] = sqrtf(v[k]);
-        p[k] = p[k] * c.decay - (m[k] / (r[k] * c.unbias + H.eps)) * c.size;
-    }
-    opt_store<FULL>(opt_at<T>(e.p, base), lane, rem, p);
-    if constexpr (BITS == 8) {
-        if constexpr (!FULL) {                   // lanes past the end do not count in the maxima (a factor that is not finite would be in them)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (lane + 64 * k >= rem) m[k] = r[k] = 0.0f;
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = base + u * 4 * OPT_BLOCK;
+        opt_load<FULL, true>(opt_at<T>(e.g, at), lane, rem, g[u]);
+        if constexpr (BITS == 8) {
+            cm[u] = opt_load_codes<FULL>(opt_at<uint8_t>(e.m, at), lane, rem);
+            cv[u] = opt_load_codes<FULL>(opt_at<uint8_t>(e.v, at), lane, rem);
+            sm[u] = *opt_at<float>(e.ms, block + 4 * u);
+            sr[u] = *opt_at<float>(e.rs, block + 4 * u);
+        } else {
+            opt_load<FULL, true>(opt_at<float>(e.m, at), lane, rem, m[u]);
+            opt_load<FULL, true>(opt_at<float>(e.v, at), lane, rem, v[u]);
         }
-        const float sm = opt_scale(m), sr = opt_scale(r);
-        opt_store_codes<FULL>(opt_at<uint8_t>(e.m, base), lane, rem, opt_encode(m, sm, false));
-        opt_store_codes<FULL>(opt_at<uint8_t>(e.v, base), lane, rem, opt_encode_root<FULL>(r, sr, base + (FULL ? 4 * lane : lane), c.t));
-        if (lane == 0) { *opt_at<float>(e.ms, block) = sm; *opt_at<float>(e.rs, block) = sr; }
-    } else {
-        opt_store<FULL>(opt_at<float>(e.m, base), lane, rem, m);
-        opt_store<FULL>(opt_at<float>(e.v, base), lane, rem, v);
+        opt_load<FULL, true>(opt_at<T>(e.p, at), lane, rem, p[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = base + u * 4 * OPT_BLOCK;
+        float r[4];
+        if constexpr (BITS == 8) {
+            opt_decode(cm[u], sm[u], m[u]);
+            opt_decode(cv[u], sr[u], v[u]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[u][k] = v[u][k] * v[u][k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            g[u][k] = g[u][k] * factor;
+            m[u][k] = m[u][k] * H.b1 + g[u][k] * H.omb1;
+            v[u][k] = v[u][k] * H.b2 + (g[u][k] * g[u][k]) * H.omb2;
+            r[k] = sqrtf(v[u][k]);
+            p[u][k] = p[u][k] * c.decay - (m[u][k] / (r[k] * c.unbias + H.eps)) * c.size;
+        }
+        if constexpr (BITS == 8) {
+            if constexpr (!FULL) {               // lanes past the end do not count in the maxima (a factor that is not finite would be in them)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (lane + 64 * k >= rem) m[u][k] = r[k] = 0.0f;
+            }
+            const float nm = opt_scale(m[u]), nr = opt_scale(r);
+            cm[u] = opt_encode(m[u], nm, false);
+            cv[u] = opt_encode_root<FULL>(r, nr, at + (FULL ? 4 * lane : lane), c.t);
+            sm[u] = nm; sr[u] = nr;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        opt_store<FULL, !(OPT_NT & 4)>(opt_at<T>(e.p, at), lane, rem, p[u]);
+        if constexpr (BITS == 8) {
+            opt_store_codes<FULL>(opt_at<uint8_t>(e.m, at), lane, rem, cm[u]);
+            opt_store_codes<FULL>(opt_at<uint8_t>(e.v, at), lane, rem, cv[u]);
+            if (lane == 0) { *opt_at<float>(e.ms, block + 4 * u) = sm[u]; *opt_at<float>(e.rs, block + 4 * u) = sr[u]; }
+        } else {
+            opt_store<FULL, true>(opt_at<float>(e.m, at), lane, rem, m[u]);
+            opt_store<FULL, true>(opt_at<float>(e.v, at), lane, rem, v[u]);
+        }
+        opt_stored();
     }
 }
 
 template <typename T, int BITS>
-__global__ __launch_bounds__(OPT_WG) void k_adamw(const OptHead* head, const OptEntry* entry, const OptCoef* coef, int n, uint32_t tiles, OptHyper H) {
+__global__ __launch_bounds__(OPT_WG) void k_adamw(const OptHead* head, const OptEntry* entry, const uint32_t* tile0, const OptCoef* coef, int n, uint32_t tiles, OptHyper H) {
     if (opt_uniform(&head->skip)) return;
     const float factor = opt_uniform(&head->factor);
     const int lane = threadIdx.x & 63;
     OptCoef c = {};
-    for (OptWalk w(entry, n, tiles); w.tile < w.tiles; w.next()) {
-        if (w.enter()) c = opt_uniform(coef + w.i);
-        const int rem = w.rem();
-        if (rem <= 0) continue;
-        if (rem == OPT_BLOCK && w.aligned<T>(1, 1, BITS == 8 ? 4 : 16)) adamw_block<T, BITS, true>(w.cur, w.base(), rem, c, H, factor, lane);
-        else adamw_block<T, BITS, false>(w.cur, w.base(), rem, c, H, factor, lane);
-    }
+    OptWalk<OPT_NB> w(entry, tile0, n, tiles);
+    opt_blocks<OPT_NB, OPT_U>(w, [&] { c = opt_uniform(coef + w.i); return w.template aligned<T>(1, 1, BITS == 8 ? 4 : 16); },
+                              [&](auto kind, int64_t base, int rem) { adamw_block<T, BITS, kind.FULL, kind.N>(w.cur, base, rem, c, H, factor, lane); });
 }
 
 // ---- global gradient norm: squares summed in fp64 (no overflow, and fp64 multiply-add runs at the rate of fp32 here), a fixed order
-template <bool FULL, typename T> __device__ __forceinline__ double opt_sumsq(const OptEntry& e, int64_t base, int rem, int lane, double s) {
-    float g[4];
-    opt_load<FULL>(opt_at<T>(e.g, base), lane, rem, g);
+template <bool FULL, int U, typename T> __device__ __forceinline__ double opt_sumsq(const OptEntry& e, int64_t base, int rem, int lane, double s) {
+    float g[U][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s = fma((double)g[k], (double)g[k], s);
+    for (int u = 0; u < U; ++u) opt_load<FULL>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s = fma((double)g[u][k], (double)g[u][k], s);
     return s;
 }
-template <typename T>
-__global__ __launch_bounds__(OPT_WG) void k_opt_sumsq(const OptEntry* entry, int n, uint32_t tiles, double* partial) {
+template <typename T, int NB>
+__global__ __launch_bounds__(OPT_WG) void k_opt_sumsq(const OptEntry* entry, const uint32_t* tile0, int n, uint32_t tiles, double* partial) {
     __shared__ double part[OPT_WG / 64];
     const int lane = threadIdx.x & 63;
     double s = 0.0;
-    for (OptWalk w(entry, n, tiles); w.tile < w.tiles; w.next()) {
-        w.enter();
-        const int rem = w.rem();
-        if (rem <= 0) continue;
-        if (rem == OPT_BLOCK && w.aligned<T>(0, 1, 0)) s = opt_sumsq<true, T>(w.cur, w.base(), rem, lane, s);
-        else s = opt_sumsq<false, T>(w.cur, w.base(), rem, lane, s);
-    }
+    OptWalk<NB> w(entry, tile0, n, tiles);
+    opt_blocks<NB, NB>(w, [&] { return w.template aligned<T>(0, 1, 0); },
+                       [&](auto kind, int64_t base, int rem) { s = opt_sumsq<kind.FULL, kind.N, T>(w.cur, base, rem, lane, s); });
     s = wave_sum_f64(s);
     if (lane == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) partial[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// norm of the unscaled gradients (count < 0: given at norm_at) and the factor they are multiplied with: min(1, max_norm / (norm + 1e-6)) / loss scale. One workgroup.
-__global__ __launch_bounds__(OPT_WG) void k_opt_norm(const double* partial, int count, const float* grad_scale, double max_norm, float* norm_at, OptHead* head) {
-    __shared__ double part[OPT_WG / 64];
+// The norm of the unscaled gradients (count < 0: given at norm_at) and the factor they are multiplied with, min(1, max_norm / (norm + 1e-6)) /
+// loss scale. One workgroup, a launch of its own: 4 us. Finishing in the last workgroup of k_opt_sumsq instead (a ticket) was no faster: 1024
+// tickets on one address take 6 us, and with 256 larger workgroups the sums themselves take 3 us more.
+__global__ __launch_bounds__(OPT_PARTIALS) void k_opt_norm(const double* partial, int count, const float* grad_scale, double max_norm, float* norm_at, OptHead* head) {
+    __shared__ double part[OPT_PARTIALS / 64];
     double s = 0.0;
-    for (int i = threadIdx.x; i < count; i += OPT_WG) s += partial[i];
+    for (int i = threadIdx.x; i < count; i += OPT_PARTIALS) s += partial[i];
     s = wave_sum_f64(s);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
+        double sum = 0.0;
+        for (int k = 0; k < OPT_PARTIALS / 64; ++k) sum += part[k];
         const double scale = grad_scale ? (double)*grad_scale : 1.0;
-        const float norm = count < 0 ? *norm_at : (float)(sqrt((part[0] + part[1]) + (part[2] + part[3])) / scale);
+        const float norm = count < 0 ? *norm_at : (float)(sqrt(sum) / scale);
         const double clip = max_norm / ((double)norm + 1e-6);
         head->factor = (float)((1.0 / scale) * (clip > 1.0 ? 1.0 : clip));     // (a NaN norm gives a NaN factor)
         if (norm_at && count >= 0) *norm_at = norm;
     }
 }
 
-template <bool FULL, typename T> __device__ __forceinline__ void opt_scale_block(const OptEntry& e, int64_t base, int rem, int lane, float factor) {
-    float g[4];
-    opt_load<FULL>(opt_at<T>(e.g, base), lane, rem, g);
+template <bool FULL, int U, typename T> __device__ __forceinline__ void opt_scale_block(const OptEntry& e, int64_t base, int rem, int lane, float factor) {
+    float g[U][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) g[k] = g[k] * factor;
-    opt_store<FULL>(opt_at<T>(e.g, base), lane, rem, g);
+    for (int u = 0; u < U; ++u) opt_load<FULL>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) g[u][k] = g[u][k] * factor;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) opt_store<FULL>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
+    opt_stored();
 }
 template <typename T>
-__global__ __launch_bounds__(OPT_WG) void k_opt_scale(const OptHead* head, const OptEntry* entry, int n, uint32_t tiles) {
+__global__ __launch_bounds__(OPT_WG) void k_opt_scale(const OptHead* head, const OptEntry* entry, const uint32_t* tile0, int n, uint32_t tiles) {
     const float factor = opt_uniform(&head->factor);
     if (factor == 1.0f) return;                  // nothing to clip: x * 1 is x for every x
     const int lane = threadIdx.x & 63;
-    for (OptWalk w(entry, n, tiles); w.tile < w.tiles; w.next()) {
-        w.enter();
-        const int rem = w.rem();
-        if (rem <= 0) continue;
-        if (rem == OPT_BLOCK && w.aligned<T>(0, 1, 0)) opt_scale_block<true, T>(w.cur, w.base(), rem, lane, factor);
-        else opt_scale_block<false, T>(w.cur, w.base(), rem, lane, factor);
-    }
+    OptWalk<OPT_CLIP_NB> w(entry, tile0, n, tiles);
+    opt_blocks<OPT_CLIP_NB, 2>(w, [&] { return w.template aligned<T>(0, 1, 0); },
+                               [&](auto kind, int64_t base, int rem) { opt_scale_block<kind.FULL, kind.N, T>(w.cur, base, rem, lane, factor); });
 }
 
 // ---- fp32 moments (p: exp_avg, g: exp_avg_sq) <-> 8-bit moments
@@ -360,8 +449,8 @@ template <bool FULL, bool WRITE> __device__ __forceinline__ void opt_state8_bloc
     const int64_t block = base / OPT_BLOCK;
     float m[4], v[4];
     if constexpr (WRITE) {
-        opt_load<FULL>(opt_at<float>(e.p, base), lane, rem, m);
-        opt_load<FULL>(opt_at<float>(e.g, base), lane, rem, v);
+        opt_load<FULL, true>(opt_at<float>(e.p, base), lane, rem, m);
+        opt_load<FULL, true>(opt_at<float>(e.g, base), lane, rem, v);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = sqrtf(v[k]);
         const float sm = opt_scale(m), sr = opt_scale(v);
@@ -375,102 +464,126 @@ template <bool FULL, bool WRITE> __device__ __forceinline__ void opt_state8_bloc
         opt_decode(cv, *opt_at<float>(e.rs, block), v);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = v[k] * v[k];
-        opt_store<FULL>(opt_at<float>(e.p, base), lane, rem, m);
-        opt_store<FULL>(opt_at<float>(e.g, base), lane, rem, v);
+        __builtin_amdgcn_sched_barrier(0);
+        opt_store<FULL, true>(opt_at<float>(e.p, base), lane, rem, m);
+        opt_store<FULL, true>(opt_at<float>(e.g, base), lane, rem, v);
+        opt_stored();
     }
 }
 template <bool WRITE>
-__global__ __launch_bounds__(OPT_WG) void k_opt_state8(const OptEntry* entry, int n, uint32_t tiles) {
+__global__ __launch_bounds__(OPT_WG) void k_opt_state8(const OptEntry* entry, const uint32_t* tile0, int n, uint32_t tiles) {
     const int lane = threadIdx.x & 63;
-    for (OptWalk w(entry, n, tiles); w.tile < w.tiles; w.next()) {
-        w.enter();
-        const int rem = w.rem();
-        if (rem <= 0) continue;
-        if (rem == OPT_BLOCK && w.aligned<float>(1, 1, 4)) opt_state8_block<true, WRITE>(w.cur, w.base(), rem, lane);
-        else opt_state8_block<false, WRITE>(w.cur, w.base(), rem, lane);
-    }
+    OptWalk<OPT_NB> w(entry, tile0, n, tiles);
+    opt_blocks<OPT_NB, 1>(w, [&] { return w.template aligned<float>(1, 1, 4); },
+                          [&](auto kind, int64_t base, int rem) { opt_state8_block<kind.FULL, WRITE>(w.cur, base, rem, lane); });
 }
 
 // ---- host side
 // kinds of a launch: parameter type x bits of the moments
-static inline int opt_kind(const NndetOptTensor& t) { return t.dtype * 2 + (t.state_bits == 8 ? 1 : 0); }
+static inline int opt_kind(const NndetOptTensor& t) { return t.dtype + (t.state_bits == 8 ? 3 : 0); }
 
 static size_t opt_bytes(int64_t n) {
-    return sizeof(OptHead) + 3 * OPT_PARTIALS * sizeof(double) + (size_t)n * (sizeof(OptEntry) + sizeof(OptCoef));
+    return sizeof(OptHead) + 6 * OPT_PARTIALS * sizeof(double) + (size_t)n * (sizeof(OptEntry) + sizeof(OptCoef) + sizeof(uint32_t));
 }
 extern "C" size_t nndet_opt_workspace_bytes(int32_t n) { return n < 0 ? 0 : opt_bytes(n); }
 
 struct OptPlan {                                 // the tensors of a call in the order of their kinds, as they lie in the table
-    OptHead* head; double* partial; OptEntry* entry; OptCoef* coef;
+    OptHead* head; double* partial; OptEntry* entry; OptCoef* coef; uint32_t* tile0;
     int first[7];                                // entries of kind k: first[k] .. first[k + 1]
     int64_t tiles[6];
 };
 
-// Checks the tensors, lays the workspace out and launches k_opt_table. `need`: bit 0 param, 1 grad, 2 moments (scales with 8 bits).
-static int opt_begin(const NndetOptTensor* t, int32_t n, int need, OptTableArgs& A, void* ws, size_t ws_bytes, OptPlan& P, hipStream_t st) {
-    if (n < 0 || (n > 0 && !t) || n >= (1 << 24)) return NNDET_EINVAL;
-    if (!ws || ((uintptr_t)ws & 15)) return NNDET_EINVAL;
-    if (ws_bytes < opt_bytes(n)) return NNDET_EWORKSPACE;
-    P.head = (OptHead*)ws;
-    P.partial = (double*)(P.head + 1);
-    P.entry = (OptEntry*)(P.partial + 3 * OPT_PARTIALS);
-    P.coef = (OptCoef*)(P.entry + n);
-    for (int i = 0; i < n; ++i) {
-        if (t[i].dtype < 0 || t[i].dtype > 2 || (t[i].state_bits != 32 && t[i].state_bits != 8)) return NNDET_EINVAL;
-        if (t[i].numel < 0 || t[i].numel >= (int64_t)1 << 40 || t[i].slot < 0 || t[i].slot >= (1 << 24)) return NNDET_EINVAL;
-        if (t[i].numel == 0) continue;
-        if (((need & 1) && !t[i].param) || ((need & 2) && !t[i].grad) || ((need & 4) && (!t[i].exp_avg || !t[i].exp_avg_sq))) return NNDET_EINVAL;
-        if ((need & 4) && t[i].state_bits == 8 && (!t[i].exp_avg_scale || !t[i].root_scale)) return NNDET_EINVAL;
-    }
-    A.head = P.head; A.first = 1; A.n = 0;
-    int at = 0;
-    for (int k = 0; k < 6; ++k) {
+struct OptScalars { int32_t* steps; const float *lr_ptr, *found_inf, *grad_scale; double lr, b1, b2; };
+
+// k_opt_table for the tensors of kinds k0 .. k0 + 2 (PTRS as their moments need); `head`: the first launch also writes the head.
+template <int PTRS>
+static int opt_table(const NndetOptTensor* t, int32_t n, const OptScalars& S, int nb, int k0, bool head, OptPlan& P, hipStream_t st) {
+    OptTableArgs<PTRS> A;
+    memset(&A, 0, offsetof(OptTableArgs<PTRS>, a));
+    A.head = P.head; A.steps = S.steps; A.lr_ptr = S.lr_ptr; A.found_inf = S.found_inf; A.grad_scale = S.grad_scale;
+    A.lr = S.lr; A.log2_b1 = log2(S.b1); A.log2_b2 = log2(S.b2); A.first = head;
+    int at = P.first[k0];
+    for (int k = k0; k < k0 + 3; ++k) {
         P.first[k] = at;
         int64_t tiles = 0;
-        for (int i = 0; i < n; ++i) {
-            if (opt_kind(t[i]) != k || (t[i].numel == 0 && !A.steps)) continue;
-            OptArg& a = A.a[A.n++];
-            a.p = t[i].param; a.g = t[i].grad; a.m = t[i].exp_avg; a.v = t[i].exp_avg_sq; a.ms = t[i].exp_avg_scale; a.rs = t[i].root_scale;
-            a.numel_slot = (uint64_t)t[i].numel | ((uint64_t)t[i].slot << 40);
-            a.wd = (float)t[i].weight_decay;
-            a.tile0 = (uint32_t)tiles;
-            tiles += ceil_div64(t[i].numel, OPT_TILE);
-            if (tiles >= ((int64_t)1 << 32) - 65536) return NNDET_EINVAL;       // (a walk steps past the last tile)
-            ++at;
-            if (A.n == OPT_ARGS) {
-                A.entry = P.entry + at - A.n; A.coef = P.coef + at - A.n;
-                k_opt_table<<<1, 64, 0, st>>>(A);
+        for (int i = 0; i <= n; ++i) {
+            if (i < n && (opt_kind(t[i]) != k || (t[i].numel == 0 && !S.steps))) continue;
+            if (i < n) {
+                OptArg<PTRS>& a = A.a[A.n++];
+                const uint64_t p[6] = {(uint64_t)t[i].param, (uint64_t)t[i].grad, (uint64_t)t[i].exp_avg, (uint64_t)t[i].exp_avg_sq,
+                                       (uint64_t)t[i].exp_avg_scale, (uint64_t)t[i].root_scale};
+                for (int q = 0; q < PTRS; ++q) {
+                    if (p[q] >> 48) return NNDET_EINVAL;
+                    a.lo[q] = (uint32_t)p[q]; a.hi[q] = (uint16_t)(p[q] >> 32);
+                }
+                a.numel_lo = (uint32_t)t[i].numel; a.numel_hi_slot = (uint32_t)(t[i].numel >> 32) | (uint32_t)t[i].slot << 8;
+                a.wd = (float)t[i].weight_decay;
+                a.tile0 = (uint32_t)tiles;
+                tiles += ceil_div64(t[i].numel, nb * 4 * OPT_BLOCK);
+                if (tiles >= ((int64_t)1 << 32) - OPT_GRID) return NNDET_EINVAL;       // (a walk steps past the last tile)
+                ++at;
+            }
+            const bool end = i == n && k == k0 + 2;
+            if (A.n == OptTableArgs<PTRS>::MOST || (end && (A.n || A.first))) {
+                A.entry = P.entry + at - A.n; A.coef = P.coef + at - A.n; A.tile0 = P.tile0 + at - A.n;
+                k_opt_table<PTRS><<<1, 128, 0, st>>>(A);
                 LAUNCH_CHECK();
                 A.n = 0; A.first = 0;
             }
         }
         P.tiles[k] = tiles;
     }
-    P.first[6] = at;
-    if (A.n || A.first) {
-        A.entry = P.entry + at - A.n; A.coef = P.coef + at - A.n;
-        k_opt_table<<<1, 64, 0, st>>>(A);
-        LAUNCH_CHECK();
+    P.first[k0 + 3] = at;
+    return 0;
+}
+
+// Checks the tensors, lays the workspace out and writes the table. `need`: bit 0 param, 1 grad, 2 moments (scales with 8 bits).
+static int opt_begin(const NndetOptTensor* t, int32_t n, int need, const OptScalars& S, int nb, void* ws, size_t ws_bytes, OptPlan& P, hipStream_t st) {
+    if (n < 0 || (n > 0 && !t) || n >= (1 << 24)) return NNDET_EINVAL;
+    if (!ws || ((uintptr_t)ws & 15)) return NNDET_EINVAL;
+    if (ws_bytes < opt_bytes(n)) return NNDET_EWORKSPACE;
+    P.head = (OptHead*)ws;
+    P.partial = (double*)(P.head + 1);
+    P.entry = (OptEntry*)(P.partial + 6 * OPT_PARTIALS);
+    P.coef = (OptCoef*)(P.entry + n);
+    P.tile0 = (uint32_t*)(P.coef + n);
+    bool any8 = false;
+    for (int i = 0; i < n; ++i) {
+        if (t[i].dtype < 0 || t[i].dtype > 2 || (t[i].state_bits != 32 && t[i].state_bits != 8)) return NNDET_EINVAL;
+        if (t[i].numel < 0 || t[i].numel >= (int64_t)1 << 40 || t[i].slot < 0 || t[i].slot >= (1 << 24)) return NNDET_EINVAL;
+        any8 |= t[i].state_bits == 8;
+        if (t[i].numel == 0) continue;
+        if (((need & 1) && !t[i].param) || ((need & 2) && !t[i].grad) || ((need & 4) && (!t[i].exp_avg || !t[i].exp_avg_sq))) return NNDET_EINVAL;
+        if ((need & 4) && t[i].state_bits == 8 && (!t[i].exp_avg_scale || !t[i].root_scale)) return NNDET_EINVAL;
     }
+    P.first[0] = 0;
+    bool any32 = n == 0;
+    for (int i = 0; i < n && !any32; ++i) any32 = t[i].state_bits == 32;
+    int rc = 0;
+    if (any32) rc = opt_table<4>(t, n, S, nb, 0, true, P, st);
+    else for (int k = 0; k < 4; ++k) { P.first[k] = 0; if (k < 3) P.tiles[k] = 0; }
+    if (rc) return rc;
+    if (any8) return opt_table<6>(t, n, S, nb, 3, !any32, P, st);
+    for (int k = 3; k < 7; ++k) { P.first[k] = P.first[3]; if (k < 6) P.tiles[k] = 0; }
     return 0;
 }
 
 static inline unsigned opt_grid(int64_t tiles, int most) { return (unsigned)(tiles < most ? tiles : most); }
 
-static int opt_norm(const OptPlan& P, const float* grad_scale, double max_norm, float* norm, bool given, hipStream_t st) {
+template <int NB> static int opt_norm(const OptPlan& P, const float* grad_scale, double max_norm, float* norm, bool given, hipStream_t st) {
     int count = 0;
     for (int k = 0; k < 6 && !given; ++k) {
         if (!P.tiles[k]) continue;
-        const unsigned g = opt_grid(P.tiles[k], OPT_PARTIALS / 2);
+        const unsigned g = opt_grid(P.tiles[k], OPT_PARTIALS);
         const OptEntry* e = P.entry + P.first[k];
         const int n = P.first[k + 1] - P.first[k];
-#define OPT_CALL(T) (k_opt_sumsq<T><<<g, OPT_WG, 0, st>>>(e, n, (uint32_t)P.tiles[k], P.partial + count))
-        NNDET_DISPATCH_DTYPE(k >> 1, OPT_CALL);
+#define OPT_CALL(T) (k_opt_sumsq<T, NB><<<g, OPT_WG, 0, st>>>(e, P.tile0 + P.first[k], n, (uint32_t)P.tiles[k], P.partial + count))
+        NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL);
 #undef OPT_CALL
         LAUNCH_CHECK();
         count += (int)g;
     }
-    k_opt_norm<<<1, OPT_WG, 0, st>>>(P.partial, given ? -1 : count, grad_scale, max_norm, norm, P.head);
+    k_opt_norm<<<1, OPT_PARTIALS, 0, st>>>(P.partial, given ? -1 : count, grad_scale, max_norm, norm, P.head);
     LAUNCH_CHECK();
     return 0;
 }
@@ -479,15 +592,12 @@ extern "C" int nndet_adamw_step(const NndetOptTensor* tensors, int32_t n, const 
     if (!a || !a->steps || !(a->beta1 >= 0.0 && a->beta1 < 1.0) || !(a->beta2 >= 0.0 && a->beta2 < 1.0) || !(a->eps >= 0.0)) return NNDET_EINVAL;
     if (a->max_norm != a->max_norm || (a->norm_given && (!a->norm || a->max_norm < 0.0))) return NNDET_EINVAL;
     hipStream_t st = as_stream(stream);
-    OptTableArgs A;
-    memset(&A, 0, sizeof(A));
-    A.steps = a->steps; A.lr_ptr = a->lr_device; A.found_inf = a->found_inf; A.grad_scale = a->grad_scale;
-    A.lr = a->lr; A.b1 = a->beta1; A.b2 = a->beta2;
+    const OptScalars S = {a->steps, a->lr_device, a->found_inf, a->grad_scale, a->lr, a->beta1, a->beta2};
     OptPlan P;
-    int rc = opt_begin(tensors, n, 7, A, workspace, workspace_bytes, P, st);
+    int rc = opt_begin(tensors, n, 7, S, OPT_NB, workspace, workspace_bytes, P, st);
     if (rc) return rc;
     if (a->max_norm >= 0.0) {
-        rc = opt_norm(P, a->grad_scale, a->max_norm, a->norm, a->norm_given != 0, st);
+        rc = opt_norm<OPT_NB>(P, a->grad_scale, a->max_norm, a->norm, a->norm_given != 0, st);
         if (rc) return rc;
     }
     const OptHyper H = {(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps};
@@ -497,10 +607,10 @@ extern "C" int nndet_adamw_step(const NndetOptTensor* tensors, int32_t n, const 
         const OptEntry* e = P.entry + P.first[k];
         const OptCoef* c = P.coef + P.first[k];
         const int m = P.first[k + 1] - P.first[k];
-#define OPT_CALL8(T) (k_adamw<T, 8><<<g, OPT_WG, 0, st>>>(P.head, e, c, m, (uint32_t)P.tiles[k], H))
-#define OPT_CALL32(T) (k_adamw<T, 32><<<g, OPT_WG, 0, st>>>(P.head, e, c, m, (uint32_t)P.tiles[k], H))
-        if (k & 1) NNDET_DISPATCH_DTYPE(k >> 1, OPT_CALL8);
-        else NNDET_DISPATCH_DTYPE(k >> 1, OPT_CALL32);
+#define OPT_CALL8(T) (k_adamw<T, 8><<<g, OPT_WG, 0, st>>>(P.head, e, P.tile0 + P.first[k], c, m, (uint32_t)P.tiles[k], H))
+#define OPT_CALL32(T) (k_adamw<T, 32><<<g, OPT_WG, 0, st>>>(P.head, e, P.tile0 + P.first[k], c, m, (uint32_t)P.tiles[k], H))
+        if (k >= 3) NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL8);
+        else NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL32);
 #undef OPT_CALL8
 #undef OPT_CALL32
         LAUNCH_CHECK();
@@ -511,20 +621,19 @@ extern "C" int nndet_adamw_step(const NndetOptTensor* tensors, int32_t n, const 
 extern "C" int nndet_grad_clip(const NndetOptTensor* tensors, int32_t n, double max_norm, const float* grad_scale, float* norm_out, void* workspace, size_t workspace_bytes, void* stream) {
     if (max_norm != max_norm || !norm_out || (grad_scale && max_norm >= 0.0)) return NNDET_EINVAL;
     hipStream_t st = as_stream(stream);
-    OptTableArgs A;
-    memset(&A, 0, sizeof(A));
+    const OptScalars S = {nullptr, nullptr, nullptr, nullptr, 0.0, 0.0, 0.0};
     OptPlan P;
-    int rc = opt_begin(tensors, n, 2, A, workspace, workspace_bytes, P, st);
+    int rc = opt_begin(tensors, n, 2, S, OPT_CLIP_NB, workspace, workspace_bytes, P, st);
     if (rc) return rc;
-    rc = opt_norm(P, grad_scale, max_norm, norm_out, false, st);
+    rc = opt_norm<OPT_CLIP_NB>(P, grad_scale, max_norm, norm_out, false, st);
     if (rc || max_norm < 0.0) return rc;         // the norm alone
     for (int k = 0; k < 6; ++k) {
         if (!P.tiles[k]) continue;
         const unsigned g = opt_grid(P.tiles[k], OPT_GRID);
         const OptEntry* e = P.entry + P.first[k];
         const int m = P.first[k + 1] - P.first[k];
-#define OPT_CALL(T) (k_opt_scale<T><<<g, OPT_WG, 0, st>>>(P.head, e, m, (uint32_t)P.tiles[k]))
-        NNDET_DISPATCH_DTYPE(k >> 1, OPT_CALL);
+#define OPT_CALL(T) (k_opt_scale<T><<<g, OPT_WG, 0, st>>>(P.head, e, P.tile0 + P.first[k], m, (uint32_t)P.tiles[k]))
+        NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL);
 #undef OPT_CALL
         LAUNCH_CHECK();
     }
@@ -535,17 +644,16 @@ extern "C" int nndet_adam_state8(const NndetOptTensor* tensors, int32_t n, int32
     for (int i = 0; tensors && i < n; ++i)
         if (tensors[i].dtype != NNDET_F32 || tensors[i].state_bits != 8) return NNDET_EINVAL;
     hipStream_t st = as_stream(stream);
-    OptTableArgs A;
-    memset(&A, 0, sizeof(A));
+    const OptScalars S = {nullptr, nullptr, nullptr, nullptr, 0.0, 0.0, 0.0};
     OptPlan P;
-    int rc = opt_begin(tensors, n, 7, A, workspace, workspace_bytes, P, st);
+    int rc = opt_begin(tensors, n, 7, S, OPT_NB, workspace, workspace_bytes, P, st);
     if (rc) return rc;
-    const int k = NNDET_F32 * 2 + 1;
+    const int k = NNDET_F32 + 3;
     if (!P.tiles[k]) return 0;
     const unsigned g = opt_grid(P.tiles[k], OPT_GRID);
     const int m = P.first[k + 1] - P.first[k];
-    if (write) k_opt_state8<true><<<g, OPT_WG, 0, st>>>(P.entry + P.first[k], m, (uint32_t)P.tiles[k]);
-    else k_opt_state8<false><<<g, OPT_WG, 0, st>>>(P.entry + P.first[k], m, (uint32_t)P.tiles[k]);
+    if (write) k_opt_state8<true><<<g, OPT_WG, 0, st>>>(P.entry + P.first[k], P.tile0 + P.first[k], m, (uint32_t)P.tiles[k]);
+    else k_opt_state8<false><<<g, OPT_WG, 0, st>>>(P.entry + P.first[k], P.tile0 + P.first[k], m, (uint32_t)P.tiles[k]);
     LAUNCH_CHECK();
     return 0;
 }

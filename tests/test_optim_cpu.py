@@ -109,8 +109,8 @@ def test_dense_and_order():
 def test_words_are_the_structs():
     wd = struct.unpack("q", struct.pack("d", 0.25))[0]
     w = O._words(2, [11, 21], [12, 22], [13, 23], [14, 24], [15, 25], [16, 26], [17, 27], [wd, wd], [5 | (L.BF16 << 32) | (8 << 48), 6 | (L.F16 << 32) | (32 << 48)])
-    assert w.itemsize * len(w) == 2 * C.sizeof(L.NndetOptTensor)
-    t = (L.NndetOptTensor * 2).from_buffer(w)
+    assert len(w) == 2 * C.sizeof(L.NndetOptTensor)
+    t = (L.NndetOptTensor * 2).from_buffer_copy(w)
     assert (t[1].param, t[1].grad, t[1].exp_avg, t[1].exp_avg_sq, t[1].exp_avg_scale, t[1].root_scale, t[1].numel) == (21, 22, 23, 24, 25, 26, 27)
     assert t[0].weight_decay == 0.25 and (t[0].slot, t[0].dtype, t[0].state_bits) == (5, L.BF16, 8) and (t[1].slot, t[1].dtype, t[1].state_bits) == (6, L.F16, 32)
 
