@@ -716,7 +716,7 @@ typedef struct NndetOptTensor {
     int16_t state_bits;     /* 32 or 8 */
 } NndetOptTensor;
 typedef struct NndetAdamw {
-    double lr, beta1, beta2, eps;
+    double lr, beta1, beta2, eps;   /* betas in [0, 1); eps 0 or a normal fp32 number */
     double max_norm;            /* >= 0: multiply the gradients by min(1, max_norm / (norm + 1e-6)) on the way; < 0: no clipping */
     const float* lr_device;     /* not NULL: the rate is read there instead (a captured step follows a schedule) */
     const float* grad_scale;    /* not NULL: the gradients carry this loss scale (torch.amp.GradScaler); they are divided by it */

@@ -3,22 +3,27 @@
 //
 // A call takes n tensors of any sizes. k_opt_table copies their addresses out of the kernel arguments into a table in the workspace (64 B
 // a tensor, up to 99 of them a launch, so that every later kernel is ONE launch whatever n is), advances the step counts and works out what
-// is the same for a whole tensor. Then one launch per storage kind walks over tiles of 1024 consecutive elements of a tensor; no tile spans
-// two tensors. A wave owns 256 consecutive elements of its tile, which is also the block that shares a scale of the 8-bit moments: the
-// block maximum never leaves the wave.
+// is the same for a whole tensor. Then one launch per storage kind (type of the parameters x bits of the moments) has a workgroup for each
+// tile of 2048 consecutive elements of a tensor; no tile spans two tensors. A wave owns blocks of 256 consecutive elements, which are also
+// the blocks that share a scale of the 8-bit moments: the maximum never leaves the wave. Calls of few small tensors skip the table.
 //
 // AdamW, t = count + 1, g' = g * factor (factor = clip / loss scale):
 //   m = b1 m + (1 - b1) g'        v = b2 v + (1 - b2) g'^2
 //   p = p (1 - lr wd) - (lr / (1 - b1^t)) * m / (sqrt(v) * (1 - b2^t)^-1/2 + eps)
-// in fp32 with every operation rounded by itself (this file is compiled without contraction; division and square root are the IEEE ones),
-// so that the 8-bit codes do not depend on how a compiler fuses; 1 - b^t, lr / (1 - b1^t) and the factor are worked out in fp64 and rounded
-// once. Parameters and gradients in 16 bits are read to fp32 and the new parameter is rounded once, to nearest even.
+// in fp32 with every operation rounded by itself (this file is compiled without contraction), so that the 8-bit codes do not depend on how a
+// compiler fuses; 1 - b^t, lr / (1 - b1^t) and the factor are worked out in fp64 and rounded once. Parameters and gradients in 16 bits are
+// read to fp32 and the new parameter is rounded once, to nearest even.
 //
 // 8-bit moments: m and r = sqrt(v) as e4m3 codes with one fp32 scale = max |.| / 448 a block. r instead of v because e4m3 spans 2^17.8 and
 // v's range is the square of the gradients'. m is rounded to nearest even (it changes by 10 % a step, codes are 6 - 12 % apart); r changes
 // by about 0.05 % a step and would never leave its code under rounding to nearest, so it is rounded up with the probability of its distance
 // from the code below: the expected value of the stored r is r. The 16 random bits an element come from its index in the tensor and
 // t alone (opt_mix), so a step is reproducible. An r that is not zero is not stored as zero: m / (0 + eps) would be a step of any size.
+//
+// Bound: HBM. Every input is read once and every output written once, 28 B an element with fp32 moments and 16.06 B with 8-bit ones (fp32
+// parameters). Measured (k_adamw alone, fp32 parameters): 295.5 M elements 1.44 ms = 5.7 TB/s and 0.76 ms = 6.2 TB/s (a large copy on the
+// same card: 4.7 - 5.0, a large in-place product 5.9 TB/s); 19.0 M elements 77 us = 6.9 TB/s and 50 us = 6.1 TB/s (part of it stays in the
+// 256 MB cache between steps).
 #include "common.h"
 #include <math.h>
 #include <stddef.h>
@@ -26,23 +31,18 @@
 
 static constexpr int OPT_WG = 256;               // threads of a workgroup: 4 waves
 static constexpr int OPT_BLOCK = 256;            // elements of a wave's block = elements that share a scale
-#ifndef OPT_NB
-#define OPT_NB 2
-#endif
-#ifndef OPT_U
-#define OPT_U 2
-#endif
-#ifndef OPT_G
-#define OPT_G 1000000
-#endif
-#ifndef OPT_NT
-#define OPT_NT 3
-#endif
-#ifndef OPT_CLIP_NB
-#define OPT_CLIP_NB 4
-#endif
-static constexpr int OPT_PARTIALS = 1024;        // workgroups (and fp64 partial sums) of the norm per storage type
-static constexpr int OPT_GRID = OPT_G;            // workgroups of a walk over the tiles: 8 for each of the 256 CUs
+// Rounds of four blocks in a tile. 2 for the step and the moments' conversion: 8 loads a lane in flight; 1 was 4 % faster for fp32 moments of 295 M
+// elements and 8 % slower for 8-bit ones and for the norm, 4 was 5 - 10 % slower at 13 - 19 M. Clipping alone moves fewer bytes a tile: 4 (150
+// tensors of 23.6 M: 36 us of GPU time without the scaling, 42 with 2).
+static constexpr int OPT_NB = 2, OPT_CLIP_NB = 4;
+// One workgroup a tile up to this many (a grid is limited to 2^32 threads). 2048 workgroups that walk over the tiles instead were 15 - 20 % slower.
+static constexpr int OPT_GRID = 1 << 20;
+static constexpr int OPT_PARTIALS = 1024;        // workgroups (and fp64 partial sums) of the norm per storage kind
+// The kernels for few small tensors take one workgroup a tensor, and one for the norm of all. Against the table's kernels (1 to 60 tensors, us of
+// GPU time / of a call with its host time): 4000 elements 5.4 / 10.4 against 6.5 / 13.7, 8000 elements 7.4 against 6.3; norm and clipping of 60 k
+// elements in all 6.7 / 12.5 against 8.8 / 20.8, of 120 k 9.4 against 8.9.
+static constexpr int OPT_FEW = 4096;
+static constexpr int64_t OPT_FEW_TOTAL = 65536;
 
 struct OptEntry {                                // one tensor in the workspace's table
     void* p; const void* g; void* m; void* v; float* ms; float* rs;
@@ -72,22 +72,38 @@ __device__ __forceinline__ void opt_stored() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int PTRS>
-__global__ __launch_bounds__(128) void k_opt_table(const OptTableArgs<PTRS> A) {
-    const int i = threadIdx.x;
-    const bool skip = A.found_inf && *A.found_inf != 0.0f;
-    if (A.first && i == 0) {
-        A.head->skip = skip;
-        A.head->factor = A.grad_scale ? (float)(1.0 / (double)*A.grad_scale) : 1.0f;   // (the norm's kernel writes it again)
-    }
-    if (i >= A.n) return;
-    const OptArg<PTRS>& a = A.a[i];
+template <int PTRS> __device__ __forceinline__ OptEntry opt_entry(const OptArg<PTRS>& a) {
     uint64_t at[6] = {0, 0, 0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < PTRS; ++k) at[k] = a.lo[k] | (uint64_t)a.hi[k] << 32;
-    const uint64_t w[8] = {at[0], at[1], at[2], at[3], at[4], at[5], a.numel_lo | (uint64_t)(a.numel_hi_slot & 0xffu) << 32, 0};
+    return {(void*)at[0], (const void*)at[1], (void*)at[2], (void*)at[3], (float*)at[4], (float*)at[5],
+            (int64_t)(a.numel_lo | (uint64_t)(a.numel_hi_slot & 0xffu) << 32), 0};
+}
+template <int PTRS> __device__ __forceinline__ OptCoef opt_coef(const OptTableArgs<PTRS>& A, float wd, int32_t t) {
+    const double lr = A.lr_ptr ? (double)*A.lr_ptr : A.lr;
+    OptCoef c;
+    c.size = (float)(lr / (1.0 - exp2((double)t * A.log2_b1)));
+    c.unbias = (float)(1.0 / sqrt(1.0 - exp2((double)t * A.log2_b2)));
+    c.decay = (float)(1.0 - lr * (double)wd);
+    c.t = (uint32_t)t;
+    return c;
+}
+template <int PTRS> __device__ __forceinline__ bool opt_skip(const OptTableArgs<PTRS>& A) { return A.found_inf && *A.found_inf != 0.0f; }
+template <int PTRS> __device__ __forceinline__ float opt_factor(const OptTableArgs<PTRS>& A) { return A.grad_scale ? (float)(1.0 / (double)*A.grad_scale) : 1.0f; }
+
+template <int PTRS>
+__global__ __launch_bounds__(128) void k_opt_table(const OptTableArgs<PTRS> A) {
+    const int i = threadIdx.x;
+    const bool skip = opt_skip(A);
+    if (A.first && i == 0) {
+        A.head->skip = skip;
+        A.head->factor = opt_factor(A);          // (the norm's kernel writes it again)
+    }
+    if (i >= A.n) return;
+    const OptArg<PTRS>& a = A.a[i];
+    const OptEntry e = opt_entry(a);
     u32x4 v[4];
-    __builtin_memcpy(v, w, sizeof(v));
+    __builtin_memcpy(v, &e, sizeof(v));
     u32x4* to = (u32x4*)(A.entry + i);
     A.tile0[i] = a.tile0;
     __builtin_amdgcn_sched_barrier(0);
@@ -98,13 +114,7 @@ __global__ __launch_bounds__(128) void k_opt_table(const OptTableArgs<PTRS> A) {
     const uint32_t slot = a.numel_hi_slot >> 8;
     const int32_t t = A.steps[slot] + 1;
     if (!skip) A.steps[slot] = t;
-    const double lr = A.lr_ptr ? (double)*A.lr_ptr : A.lr;
-    OptCoef c;
-    c.size = (float)(lr / (1.0 - exp2((double)t * A.log2_b1)));
-    c.unbias = (float)(1.0 / sqrt(1.0 - exp2((double)t * A.log2_b2)));
-    c.decay = (float)(1.0 - lr * (double)a.wd);
-    c.t = (uint32_t)t;
-    A.coef[i] = c;
+    A.coef[i] = opt_coef(A, a.wd, t);
     opt_stored();
 }
 
@@ -137,8 +147,16 @@ __device__ __forceinline__ int opt_find(const uint32_t* tile0, int n, uint32_t t
     return __builtin_amdgcn_readfirstlane(found - 1);
 }
 
-// The walk of a workgroup over the tiles blockIdx.x, blockIdx.x + gridDim.x, ...: at any time the chip works on neighbouring addresses (few
-// pages, few open DRAM rows). The tensor is looked up again only when the walk leaves it.
+// whether four elements of g (and p) of `size` bytes each are aligned vectors, and m and v are aligned to `state` bytes (0: not used)
+__device__ __forceinline__ bool opt_vectors(const OptEntry& e, int size, bool params, int state) {
+    uintptr_t a = (uintptr_t)e.g & (4 * size - 1);
+    if (params) a |= (uintptr_t)e.p & (4 * size - 1);
+    if (state) a |= ((uintptr_t)e.m | (uintptr_t)e.v) & (state - 1);
+    return a == 0;
+}
+
+// The walk of a workgroup over the tiles blockIdx.x, blockIdx.x + gridDim.x, ... (one tile alone where the grid covers them): at any time the
+// chip works on neighbouring addresses. The tensor is looked up again only when the walk leaves it.
 template <int NB> struct OptWalk {
     static constexpr int TILE = NB * 4 * OPT_BLOCK;
     const OptEntry* e; const uint32_t* tile0; int n; uint32_t tiles, tile, start, end;
@@ -161,28 +179,24 @@ template <int NB> struct OptWalk {
         const int64_t r = cur.numel - base();
         return r < TILE ? (int)r : TILE;                  // (a tile is not empty: r > -TILE)
     }
-    // whether four elements of p (wp) and g (wg) are aligned vectors of T, and m and v are aligned to ms bytes (0: not used)
-    template <typename T> __device__ __forceinline__ bool aligned(int wp, int wg, int ms) const {
-        uintptr_t a = 0;
-        if (wp) a |= (uintptr_t)cur.p & (4 * sizeof(T) - 1);
-        if (wg) a |= (uintptr_t)cur.g & (4 * sizeof(T) - 1);
-        if (ms) a |= ((uintptr_t)cur.m | (uintptr_t)cur.v) & (ms - 1);
-        return a == 0;
-    }
 };
 
 // ---- four elements a lane. FULL (a whole block of an aligned tensor): one vector a lane, elements 4 lane + 0..3; else element by element,
 // lane + 64 k while that is below rem, zeros behind. The addresses come out of the table, so the compiler is told that they are global.
 template <typename T> using OptPtr = __attribute__((address_space(1))) T*;
 template <typename T> __device__ __forceinline__ OptPtr<T> opt_at(const void* p, int64_t i) { return (OptPtr<T>)(uintptr_t)p + i; }
+// STREAM: nontemporal. What a step reads and writes once would only push the rest out of the caches: with plain accesses the step of 295 M
+// parameters takes 1.54 ms instead of 1.40 (nontemporal loads or stores alone: 1.57 - 1.60), reading the 8-bit moments 0.58 instead of 0.53 ms.
 template <typename T> struct OptVec4;
 template <> struct OptVec4<float> { typedef f32x4 type; };
 template <> struct OptVec4<bf16_t> { typedef bf16_t type __attribute__((ext_vector_type(4))); };
 template <> struct OptVec4<f16_t> { typedef f16_t type __attribute__((ext_vector_type(4))); };
 
-template <bool FULL, bool ONCE = false, typename T> __device__ __forceinline__ void opt_load(OptPtr<T> p, int lane, int rem, float* x) {
+template <bool FULL, bool STREAM, typename T> __device__ __forceinline__ void opt_load(OptPtr<T> p, int lane, int rem, float* x) {
     if constexpr (FULL) {
-        const auto v = ONCE && (OPT_NT & 1) ? __builtin_nontemporal_load(((OptPtr<typename OptVec4<T>::type>)p) + lane) : ((OptPtr<typename OptVec4<T>::type>)p)[lane];
+        typename OptVec4<T>::type v;
+        if constexpr (STREAM) v = __builtin_nontemporal_load((OptPtr<typename OptVec4<T>::type>)p + lane);
+        else v = ((OptPtr<typename OptVec4<T>::type>)p)[lane];
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = Elem<T>::ld(v[k]);
     } else {
@@ -190,12 +204,12 @@ template <bool FULL, bool ONCE = false, typename T> __device__ __forceinline__ v
         for (int k = 0; k < 4; ++k) x[k] = lane + 64 * k < rem ? Elem<T>::ld(p[lane + 64 * k]) : 0.0f;
     }
 }
-template <bool FULL, bool ONCE = false, typename T> __device__ __forceinline__ void opt_store(OptPtr<T> p, int lane, int rem, const float* x) {
+template <bool FULL, bool STREAM, typename T> __device__ __forceinline__ void opt_store(OptPtr<T> p, int lane, int rem, const float* x) {
     if constexpr (FULL) {
         typename OptVec4<T>::type v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = Elem<T>::st(x[k]);
-        if (ONCE && (OPT_NT & 2)) __builtin_nontemporal_store(v, ((OptPtr<typename OptVec4<T>::type>)p) + lane);
+        if constexpr (STREAM) __builtin_nontemporal_store(v, (OptPtr<typename OptVec4<T>::type>)p + lane);
         else ((OptPtr<typename OptVec4<T>::type>)p)[lane] = v;
     } else {
 #pragma unroll
@@ -204,14 +218,14 @@ template <bool FULL, bool ONCE = false, typename T> __device__ __forceinline__ v
     }
 }
 template <bool FULL> __device__ __forceinline__ uint32_t opt_load_codes(OptPtr<uint8_t> p, int lane, int rem) {
-    if constexpr (FULL) return OPT_NT & 1 ? __builtin_nontemporal_load((OptPtr<uint32_t>)p + lane) : ((OptPtr<uint32_t>)p)[lane];
+    if constexpr (FULL) return __builtin_nontemporal_load((OptPtr<uint32_t>)p + lane);
     uint32_t c = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) c |= (lane + 64 * k < rem ? (uint32_t)p[lane + 64 * k] : 0u) << (8 * k);
     return c;
 }
 template <bool FULL> __device__ __forceinline__ void opt_store_codes(OptPtr<uint8_t> p, int lane, int rem, uint32_t c) {
-    if constexpr (FULL) { if (OPT_NT & 2) __builtin_nontemporal_store(c, (OptPtr<uint32_t>)p + lane); else ((OptPtr<uint32_t>)p)[lane] = c; return; }
+    if constexpr (FULL) { __builtin_nontemporal_store(c, (OptPtr<uint32_t>)p + lane); return; }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         if (lane + 64 * k < rem) p[lane + 64 * k] = (uint8_t)(c >> (8 * k));
@@ -237,13 +251,15 @@ __device__ __forceinline__ void opt_decode(uint32_t c, float s, float* x) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
     x[0] = lo[0] * s; x[1] = lo[1] * s; x[2] = hi[0] * s; x[3] = hi[1] * s;
 }
+// 1 / scale, 0 for a block of zeros (whose codes are then 0)
+__device__ __forceinline__ float opt_inverse(float s) { return s == 0.0f ? 0.0f : 1.0f / s; }
 __device__ __forceinline__ uint32_t opt_encode(const float* x, float s, bool root) {      // to nearest even
-    const float inv = 1.0f / s;
+    const float inv = opt_inverse(s);
     float y[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        y[k] = s > 0.0f ? x[k] * inv : 0.0f;
-        if (root && x[k] > 0.0f && s > 0.0f) y[k] = y[k] < 0x1p-9f ? 0x1p-9f : y[k];
+        y[k] = x[k] * inv;
+        if (root && x[k] > 0.0f) y[k] = y[k] < 0x1p-9f ? 0x1p-9f : y[k];
     }
     int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
@@ -259,24 +275,35 @@ __device__ __forceinline__ uint32_t opt_mix(uint32_t pair, uint32_t t) {
 // code of x / s >= 0, rounded up with the probability (in 16 bits) of its distance from the code below. Times 2^-120 the exponent field of an
 // fp32 number is e4m3's, denormals among them: adding 20 random bits below the code and cutting them off is the rounding.
 template <bool FULL> __device__ __forceinline__ uint32_t opt_encode_root(const float* x, float s, int64_t index, uint32_t t) {
-    const float inv = 1.0f / s;
+    const float inv = opt_inverse(s);
     uint32_t c = 0, bits = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int64_t i = FULL ? index + k : index + 64 * k;
         if (!FULL || !(k & 1)) bits = opt_mix((uint32_t)(i >> 1), t);
         const uint32_t u = ((FULL ? k : (int)i) & 1 ? bits >> 16 : bits & 0xffffu) * 16 + 8;
-        const float y = s > 0.0f ? x[k] * inv : 0.0f;
-        uint32_t q = (__float_as_uint(y * 0x1p-120f) + u) >> 20;
-        q = q > 0x7eu ? 0x7eu : q;
-        if (q == 0 && x[k] > 0.0f && s > 0.0f) q = 1;
-        c |= q << (8 * k);
+        const uint32_t q = (__float_as_uint(x[k] * inv * 0x1p-120f) + u) >> 20;
+        const uint32_t least = min(__float_as_uint(x[k]), 1u);           // x > 0 is not stored as 0
+        c |= min(max(q, least), 0x7eu) << (8 * k);
     }
     return c;
 }
 
-// Runs f over the blocks of the walk's tiles: f(Full<U>, base) on U whole blocks of an aligned tensor (4 * OPT_BLOCK apart), f(Part, base, rem) on
-// one block of rem elements. `enter` is called when the walk comes to another tensor, `aligned` tells whether that may use vectors.
+// Square root and quotient of the 8-bit step, which with the IEEE sequences kept its vector units busy for 73 % (19.0 M elements) to 94 % (295 M) of
+// the time: 85 instructions an element. 19 and 13 issue slots for those sequences, 11 and 8 for these: 60.5 -> 58.3 us at 19.0 M, no change at 295 M.
+// One residual step behind the hardware's reciprocal (root): correctly rounded but for about one value in 2^22.
+__device__ __forceinline__ float opt_root(float v) {
+    const float y = __builtin_amdgcn_rsqf(v), s = v * y;
+    const float r = fmaf(fmaf(-s, s, v), 0.5f * y, s);
+    return __builtin_amdgcn_classf(v, 0x100) ? r : v * 0x1p-24f;         // not a positive normal number: 0, inf and NaN are their own roots, denormals go to 0
+}
+__device__ __forceinline__ float opt_quotient(float m, float d) {       // d is not a denormal: the root is 0 or above 2^-63, and so is eps
+    const float y = __builtin_amdgcn_rcpf(d), q = m * y;
+    return __builtin_amdgcn_div_fixupf(fmaf(fmaf(-d, q, m), y, q), d, m);
+}
+
+// Runs f over the blocks of the walk's tiles: f(OptWhole<U>, base, 256) on U whole blocks of an aligned tensor (4 * OPT_BLOCK apart), f(OptPart, base,
+// rem) on one block of rem elements. `enter` is called when the walk comes to another tensor and tells whether that is aligned.
 template <int U> struct OptWhole { static constexpr bool FULL = true; static constexpr int N = U; };
 struct OptPart { static constexpr bool FULL = false; static constexpr int N = 1; };
 template <int NB, int U, typename W, typename E, typename F> __device__ __forceinline__ void opt_blocks(W& w, E enter, F f) {
@@ -336,8 +363,9 @@ __device__ __forceinline__ void adamw_block(const OptEntry& e, int64_t base, int
             g[u][k] = g[u][k] * factor;
             m[u][k] = m[u][k] * H.b1 + g[u][k] * H.omb1;
             v[u][k] = v[u][k] * H.b2 + (g[u][k] * g[u][k]) * H.omb2;
-            r[k] = sqrtf(v[u][k]);
-            p[u][k] = p[u][k] * c.decay - (m[u][k] / (r[k] * c.unbias + H.eps)) * c.size;
+            r[k] = BITS == 8 ? opt_root(v[u][k]) : sqrtf(v[u][k]);
+            const float den = r[k] * c.unbias + H.eps;
+            p[u][k] = p[u][k] * c.decay - (BITS == 8 ? opt_quotient(m[u][k], den) : m[u][k] / den) * c.size;
         }
         if constexpr (BITS == 8) {
             if constexpr (!FULL) {               // lanes past the end do not count in the maxima (a factor that is not finite would be in them)
@@ -351,7 +379,7 @@ __device__ __forceinline__ void adamw_block(const OptEntry& e, int64_t base, int
             sm[u] = nm; sr[u] = nr;
         }
         __builtin_amdgcn_sched_barrier(0);
-        opt_store<FULL, !(OPT_NT & 4)>(opt_at<T>(e.p, at), lane, rem, p[u]);
+        opt_store<FULL, true>(opt_at<T>(e.p, at), lane, rem, p[u]);
         if constexpr (BITS == 8) {
             opt_store_codes<FULL>(opt_at<uint8_t>(e.m, at), lane, rem, cm[u]);
             opt_store_codes<FULL>(opt_at<uint8_t>(e.v, at), lane, rem, cv[u]);
@@ -371,7 +399,7 @@ __global__ __launch_bounds__(OPT_WG) void k_adamw(const OptHead* head, const Opt
     const int lane = threadIdx.x & 63;
     OptCoef c = {};
     OptWalk<OPT_NB> w(entry, tile0, n, tiles);
-    opt_blocks<OPT_NB, OPT_U>(w, [&] { c = opt_uniform(coef + w.i); return w.template aligned<T>(1, 1, BITS == 8 ? 4 : 16); },
+    opt_blocks<OPT_NB, OPT_NB>(w, [&] { c = opt_uniform(coef + w.i); return opt_vectors(w.cur, sizeof(T), true, BITS == 8 ? 4 : 16); },
                               [&](auto kind, int64_t base, int rem) { adamw_block<T, BITS, kind.FULL, kind.N>(w.cur, base, rem, c, H, factor, lane); });
 }
 
@@ -379,7 +407,7 @@ __global__ __launch_bounds__(OPT_WG) void k_adamw(const OptHead* head, const Opt
 template <bool FULL, int U, typename T> __device__ __forceinline__ double opt_sumsq(const OptEntry& e, int64_t base, int rem, int lane, double s) {
     float g[U][4];
 #pragma unroll
-    for (int u = 0; u < U; ++u) opt_load<FULL>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
+    for (int u = 0; u < U; ++u) opt_load<FULL, false>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -392,7 +420,7 @@ __global__ __launch_bounds__(OPT_WG) void k_opt_sumsq(const OptEntry* entry, con
     const int lane = threadIdx.x & 63;
     double s = 0.0;
     OptWalk<NB> w(entry, tile0, n, tiles);
-    opt_blocks<NB, NB>(w, [&] { return w.template aligned<T>(0, 1, 0); },
+    opt_blocks<NB, NB>(w, [&] { return opt_vectors(w.cur, sizeof(T), false, 0); },
                        [&](auto kind, int64_t base, int rem) { s = opt_sumsq<kind.FULL, kind.N, T>(w.cur, base, rem, lane, s); });
     s = wave_sum_f64(s);
     if (lane == 0) part[threadIdx.x >> 6] = s;
@@ -400,9 +428,15 @@ __global__ __launch_bounds__(OPT_WG) void k_opt_sumsq(const OptEntry* entry, con
     if (threadIdx.x == 0) partial[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// The norm of the unscaled gradients (count < 0: given at norm_at) and the factor they are multiplied with, min(1, max_norm / (norm + 1e-6)) /
-// loss scale. One workgroup, a launch of its own: 4 us. Finishing in the last workgroup of k_opt_sumsq instead (a ticket) was no faster: 1024
-// tickets on one address take 6 us, and with 256 larger workgroups the sums themselves take 3 us more.
+// norm of the unscaled gradients from the sum of squares, and the factor they are multiplied with: min(1, max_norm / (norm + 1e-6)) / loss scale
+__device__ __forceinline__ float opt_norm_of(double sum, const float* grad_scale) { return (float)(sqrt(sum) / (grad_scale ? (double)*grad_scale : 1.0)); }
+__device__ __forceinline__ float opt_clip(float norm, const float* grad_scale, double max_norm) {
+    const double clip = max_norm / ((double)norm + 1e-6), scale = grad_scale ? (double)*grad_scale : 1.0;
+    return (float)((1.0 / scale) * (clip > 1.0 ? 1.0 : clip));           // (a NaN norm gives a NaN factor)
+}
+
+// The norm (count < 0: given at norm_at) and the factor. One workgroup, a launch of its own: 4 us. Finishing in the last workgroup of k_opt_sumsq
+// instead (a ticket) was no faster: 1024 tickets on one address take 6 us, and with 256 larger workgroups the sums themselves take 3 us more.
 __global__ __launch_bounds__(OPT_PARTIALS) void k_opt_norm(const double* partial, int count, const float* grad_scale, double max_norm, float* norm_at, OptHead* head) {
     __shared__ double part[OPT_PARTIALS / 64];
     double s = 0.0;
@@ -413,10 +447,8 @@ __global__ __launch_bounds__(OPT_PARTIALS) void k_opt_norm(const double* partial
     if (threadIdx.x == 0) {
         double sum = 0.0;
         for (int k = 0; k < OPT_PARTIALS / 64; ++k) sum += part[k];
-        const double scale = grad_scale ? (double)*grad_scale : 1.0;
-        const float norm = count < 0 ? *norm_at : (float)(sqrt(sum) / scale);
-        const double clip = max_norm / ((double)norm + 1e-6);
-        head->factor = (float)((1.0 / scale) * (clip > 1.0 ? 1.0 : clip));     // (a NaN norm gives a NaN factor)
+        const float norm = count < 0 ? *norm_at : opt_norm_of(sum, grad_scale);
+        head->factor = opt_clip(norm, grad_scale, max_norm);
         if (norm_at && count >= 0) *norm_at = norm;
     }
 }
@@ -424,14 +456,14 @@ __global__ __launch_bounds__(OPT_PARTIALS) void k_opt_norm(const double* partial
 template <bool FULL, int U, typename T> __device__ __forceinline__ void opt_scale_block(const OptEntry& e, int64_t base, int rem, int lane, float factor) {
     float g[U][4];
 #pragma unroll
-    for (int u = 0; u < U; ++u) opt_load<FULL>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
+    for (int u = 0; u < U; ++u) opt_load<FULL, false>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int k = 0; k < 4; ++k) g[u][k] = g[u][k] * factor;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < U; ++u) opt_store<FULL>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
+    for (int u = 0; u < U; ++u) opt_store<FULL, false>(opt_at<T>(e.g, base + u * 4 * OPT_BLOCK), lane, rem, g[u]);
     opt_stored();
 }
 template <typename T>
@@ -440,7 +472,7 @@ __global__ __launch_bounds__(OPT_WG) void k_opt_scale(const OptHead* head, const
     if (factor == 1.0f) return;                  // nothing to clip: x * 1 is x for every x
     const int lane = threadIdx.x & 63;
     OptWalk<OPT_CLIP_NB> w(entry, tile0, n, tiles);
-    opt_blocks<OPT_CLIP_NB, 2>(w, [&] { return w.template aligned<T>(0, 1, 0); },
+    opt_blocks<OPT_CLIP_NB, 2>(w, [&] { return opt_vectors(w.cur, sizeof(T), false, 0); },
                                [&](auto kind, int64_t base, int rem) { opt_scale_block<kind.FULL, kind.N, T>(w.cur, base, rem, lane, factor); });
 }
 
@@ -474,8 +506,84 @@ template <bool WRITE>
 __global__ __launch_bounds__(OPT_WG) void k_opt_state8(const OptEntry* entry, const uint32_t* tile0, int n, uint32_t tiles) {
     const int lane = threadIdx.x & 63;
     OptWalk<OPT_NB> w(entry, tile0, n, tiles);
-    opt_blocks<OPT_NB, 1>(w, [&] { return w.template aligned<float>(1, 1, 4); },
+    opt_blocks<OPT_NB, 1>(w, [&] { return opt_vectors(w.cur, 4, true, 4); },
                           [&](auto kind, int64_t base, int rem) { opt_state8_block<kind.FULL, WRITE>(w.cur, base, rem, lane); });
+}
+
+// ---- few small tensors: no table. The tensors are read from the kernel arguments by the kernel that works on them, one workgroup a tensor, which
+// also advances its count: one launch instead of two (with clipping two instead of four; clipping alone one instead of four). A launch costs 4 us of
+// host time and 2 - 4 us of GPU time, which is what such a call consists of.
+template <typename T, int BITS>
+__global__ __launch_bounds__(OPT_WG) void k_adamw_few(const OptTableArgs<BITS == 8 ? 6 : 4> A, OptHyper H, int clipped) {
+    if (opt_skip(A)) return;
+    const OptEntry e = opt_entry(A.a[blockIdx.x]);
+    const uint32_t slot = A.a[blockIdx.x].numel_hi_slot >> 8;
+    const int32_t t = A.steps[slot] + 1;
+    const OptCoef c = opt_coef(A, A.a[blockIdx.x].wd, t);
+    const float factor = clipped ? A.head->factor : opt_factor(A);
+    __syncthreads();                             // every wave has read the count
+    if (threadIdx.x == 0) A.steps[slot] = t;
+    const bool vec = opt_vectors(e, sizeof(T), true, BITS == 8 ? 4 : 16);
+    const int lane = threadIdx.x & 63, n = (int)e.numel;
+    for (int base = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * OPT_BLOCK; base < n; base += 4 * OPT_BLOCK) {
+        if (vec && n - base >= OPT_BLOCK) adamw_block<T, BITS, true, 1>(e, base, OPT_BLOCK, c, H, factor, lane);
+        else adamw_block<T, BITS, false, 1>(e, base, min(n - base, OPT_BLOCK), c, H, factor, lane);
+    }
+}
+
+static constexpr int OPT_FEW_WG = 1024;
+// The norm of all tensors of the call by one workgroup, a wave a tensor; SCALE: and the gradients multiplied by the factor.
+template <typename T, bool SCALE, int PTRS>
+__global__ __launch_bounds__(OPT_FEW_WG) void k_opt_norm_few(const OptTableArgs<PTRS> A, double max_norm, float* norm_at) {
+    __shared__ double part[OPT_FEW_WG / 64];
+    __shared__ float all;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    double s = 0.0;
+    for (int i = wave; i < A.n; i += OPT_FEW_WG / 64) {
+        const OptEntry e = opt_entry(A.a[i]);
+        const bool vec = opt_vectors(e, sizeof(T), false, 0);
+        const int n = (int)e.numel;
+        for (int base = 0; base < n; base += OPT_BLOCK) {
+            if (vec && n - base >= OPT_BLOCK) s = opt_sumsq<true, 1, T>(e, base, OPT_BLOCK, lane, s);
+            else s = opt_sumsq<false, 1, T>(e, base, min(n - base, OPT_BLOCK), lane, s);
+        }
+    }
+    s = wave_sum_f64(s);
+    if (lane == 0) part[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double sum = 0.0;
+        for (int k = 0; k < OPT_FEW_WG / 64; ++k) sum += part[k];
+        const float norm = opt_norm_of(sum, A.grad_scale);
+        all = opt_clip(norm, A.grad_scale, max_norm);
+        if (!SCALE) A.head->factor = all;
+        if (norm_at) *norm_at = norm;
+    }
+    if constexpr (SCALE) {
+        if (max_norm < 0.0) return;              // the norm alone
+        __syncthreads();
+        const float factor = all;
+        if (factor == 1.0f) return;
+        for (int i = wave; i < A.n; i += OPT_FEW_WG / 64) {
+            const OptEntry e = opt_entry(A.a[i]);
+            const bool vec = opt_vectors(e, sizeof(T), false, 0);
+            const int n = (int)e.numel;
+            for (int base = 0; base < n; base += OPT_BLOCK) {
+                if (vec && n - base >= OPT_BLOCK) opt_scale_block<true, 1, T>(e, base, OPT_BLOCK, lane, factor);
+                else opt_scale_block<false, 1, T>(e, base, min(n - base, OPT_BLOCK), lane, factor);
+            }
+        }
+    }
+}
+template <bool WRITE>
+__global__ __launch_bounds__(OPT_WG) void k_opt_state8_few(const OptTableArgs<6> A) {
+    const OptEntry e = opt_entry(A.a[blockIdx.x]);
+    const bool vec = opt_vectors(e, 4, true, 4);
+    const int lane = threadIdx.x & 63, n = (int)e.numel;
+    for (int base = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * OPT_BLOCK; base < n; base += 4 * OPT_BLOCK) {
+        if (vec && n - base >= OPT_BLOCK) opt_state8_block<true, WRITE>(e, base, OPT_BLOCK, lane);
+        else opt_state8_block<false, WRITE>(e, base, min(n - base, OPT_BLOCK), lane);
+    }
 }
 
 // ---- host side
@@ -495,13 +603,27 @@ struct OptPlan {                                 // the tensors of a call in the
 
 struct OptScalars { int32_t* steps; const float *lr_ptr, *found_inf, *grad_scale; double lr, b1, b2; };
 
+template <int PTRS> static void opt_scalars(const OptScalars& S, OptHead* head, OptTableArgs<PTRS>& A) {
+    memset(&A, 0, offsetof(OptTableArgs<PTRS>, a));
+    A.head = head; A.steps = S.steps; A.lr_ptr = S.lr_ptr; A.found_inf = S.found_inf; A.grad_scale = S.grad_scale;
+    A.lr = S.lr; A.log2_b1 = log2(S.b1); A.log2_b2 = log2(S.b2);
+}
+template <int PTRS> static void opt_arg(const NndetOptTensor& t, uint32_t tile0, OptArg<PTRS>& a) {
+    const uint64_t p[6] = {(uint64_t)t.param, (uint64_t)t.grad, (uint64_t)t.exp_avg, (uint64_t)t.exp_avg_sq, (uint64_t)t.exp_avg_scale, (uint64_t)t.root_scale};
+    for (int q = 0; q < PTRS; ++q) {
+        a.lo[q] = (uint32_t)p[q]; a.hi[q] = (uint16_t)(p[q] >> 32);
+    }
+    a.numel_lo = (uint32_t)t.numel; a.numel_hi_slot = (uint32_t)(t.numel >> 32) | (uint32_t)t.slot << 8;
+    a.wd = (float)t.weight_decay;
+    a.tile0 = tile0;
+}
+
 // k_opt_table for the tensors of kinds k0 .. k0 + 2 (PTRS as their moments need); `head`: the first launch also writes the head.
 template <int PTRS>
 static int opt_table(const NndetOptTensor* t, int32_t n, const OptScalars& S, int nb, int k0, bool head, OptPlan& P, hipStream_t st) {
     OptTableArgs<PTRS> A;
-    memset(&A, 0, offsetof(OptTableArgs<PTRS>, a));
-    A.head = P.head; A.steps = S.steps; A.lr_ptr = S.lr_ptr; A.found_inf = S.found_inf; A.grad_scale = S.grad_scale;
-    A.lr = S.lr; A.log2_b1 = log2(S.b1); A.log2_b2 = log2(S.b2); A.first = head;
+    opt_scalars(S, P.head, A);
+    A.first = head;
     int at = P.first[k0];
     for (int k = k0; k < k0 + 3; ++k) {
         P.first[k] = at;
@@ -509,18 +631,8 @@ static int opt_table(const NndetOptTensor* t, int32_t n, const OptScalars& S, in
         for (int i = 0; i <= n; ++i) {
             if (i < n && (opt_kind(t[i]) != k || (t[i].numel == 0 && !S.steps))) continue;
             if (i < n) {
-                OptArg<PTRS>& a = A.a[A.n++];
-                const uint64_t p[6] = {(uint64_t)t[i].param, (uint64_t)t[i].grad, (uint64_t)t[i].exp_avg, (uint64_t)t[i].exp_avg_sq,
-                                       (uint64_t)t[i].exp_avg_scale, (uint64_t)t[i].root_scale};
-                for (int q = 0; q < PTRS; ++q) {
-                    if (p[q] >> 48) return NNDET_EINVAL;
-                    a.lo[q] = (uint32_t)p[q]; a.hi[q] = (uint16_t)(p[q] >> 32);
-                }
-                a.numel_lo = (uint32_t)t[i].numel; a.numel_hi_slot = (uint32_t)(t[i].numel >> 32) | (uint32_t)t[i].slot << 8;
-                a.wd = (float)t[i].weight_decay;
-                a.tile0 = (uint32_t)tiles;
+                opt_arg(t[i], (uint32_t)tiles, A.a[A.n++]);
                 tiles += ceil_div64(t[i].numel, nb * 4 * OPT_BLOCK);
-                if (tiles >= ((int64_t)1 << 32) - OPT_GRID) return NNDET_EINVAL;       // (a walk steps past the last tile)
                 ++at;
             }
             const bool end = i == n && k == k0 + 2;
@@ -537,8 +649,8 @@ static int opt_table(const NndetOptTensor* t, int32_t n, const OptScalars& S, in
     return 0;
 }
 
-// Checks the tensors, lays the workspace out and writes the table. `need`: bit 0 param, 1 grad, 2 moments (scales with 8 bits).
-static int opt_begin(const NndetOptTensor* t, int32_t n, int need, const OptScalars& S, int nb, void* ws, size_t ws_bytes, OptPlan& P, hipStream_t st) {
+// Checks the tensors (all of them, before anything is launched) and lays the workspace out. `need`: bit 0 param, 1 grad, 2 moments (scales with 8 bits).
+static int opt_check(const NndetOptTensor* t, int32_t n, int need, void* ws, size_t ws_bytes, OptPlan& P) {
     if (n < 0 || (n > 0 && !t) || n >= (1 << 24)) return NNDET_EINVAL;
     if (!ws || ((uintptr_t)ws & 15)) return NNDET_EINVAL;
     if (ws_bytes < opt_bytes(n)) return NNDET_EWORKSPACE;
@@ -547,18 +659,25 @@ static int opt_begin(const NndetOptTensor* t, int32_t n, int need, const OptScal
     P.entry = (OptEntry*)(P.partial + 6 * OPT_PARTIALS);
     P.coef = (OptCoef*)(P.entry + n);
     P.tile0 = (uint32_t*)(P.coef + n);
-    bool any8 = false;
+    int64_t tiles = 0;
     for (int i = 0; i < n; ++i) {
         if (t[i].dtype < 0 || t[i].dtype > 2 || (t[i].state_bits != 32 && t[i].state_bits != 8)) return NNDET_EINVAL;
         if (t[i].numel < 0 || t[i].numel >= (int64_t)1 << 40 || t[i].slot < 0 || t[i].slot >= (1 << 24)) return NNDET_EINVAL;
-        any8 |= t[i].state_bits == 8;
+        const uint64_t any = (uint64_t)t[i].param | (uint64_t)t[i].grad | (uint64_t)t[i].exp_avg | (uint64_t)t[i].exp_avg_sq | (uint64_t)t[i].exp_avg_scale | (uint64_t)t[i].root_scale;
+        tiles += ceil_div64(t[i].numel, 4 * OPT_BLOCK);
+        if (any >> 48 || tiles >= ((int64_t)1 << 32) - OPT_GRID) return NNDET_EINVAL;      // (a walk steps past the last tile)
         if (t[i].numel == 0) continue;
         if (((need & 1) && !t[i].param) || ((need & 2) && !t[i].grad) || ((need & 4) && (!t[i].exp_avg || !t[i].exp_avg_sq))) return NNDET_EINVAL;
         if ((need & 4) && t[i].state_bits == 8 && (!t[i].exp_avg_scale || !t[i].root_scale)) return NNDET_EINVAL;
     }
+    return 0;
+}
+
+// Writes the table.
+static int opt_begin(const NndetOptTensor* t, int32_t n, const OptScalars& S, int nb, OptPlan& P, hipStream_t st) {
+    bool any8 = false, any32 = n == 0;
+    for (int i = 0; i < n; ++i) (t[i].state_bits == 8 ? any8 : any32) = true;
     P.first[0] = 0;
-    bool any32 = n == 0;
-    for (int i = 0; i < n && !any32; ++i) any32 = t[i].state_bits == 32;
     int rc = 0;
     if (any32) rc = opt_table<4>(t, n, S, nb, 0, true, P, st);
     else for (int k = 0; k < 4; ++k) { P.first[k] = 0; if (k < 3) P.tiles[k] = 0; }
@@ -566,6 +685,22 @@ static int opt_begin(const NndetOptTensor* t, int32_t n, int need, const OptScal
     if (any8) return opt_table<6>(t, n, S, nb, 3, !any32, P, st);
     for (int k = 3; k < 7; ++k) { P.first[k] = P.first[3]; if (k < 6) P.tiles[k] = 0; }
     return 0;
+}
+
+// The arguments of the few-tensor kernels, if the call is one for them: one kind, no more tensors than the arguments hold, none above OPT_FEW
+// elements, `total` elements at most in all. Returns the kind, or -1 if it is not.
+template <int PTRS>
+static int opt_few(const NndetOptTensor* t, int32_t n, int64_t total, const OptScalars& S, OptPlan& P, OptTableArgs<PTRS>& A) {
+    if (n < 1 || n > OptTableArgs<PTRS>::MOST || (PTRS == 6) != (t[0].state_bits == 8)) return -1;
+    const int kind = opt_kind(t[0]);
+    for (int i = 0; i < n; ++i) {
+        total -= t[i].numel;
+        if (opt_kind(t[i]) != kind || t[i].numel > OPT_FEW || total < 0) return -1;
+    }
+    opt_scalars(S, P.head, A);
+    A.n = n;
+    for (int i = 0; i < n; ++i) opt_arg(t[i], 0, A.a[i]);
+    return kind;
 }
 
 static inline unsigned opt_grid(int64_t tiles, int most) { return (unsigned)(tiles < most ? tiles : most); }
@@ -588,19 +723,39 @@ template <int NB> static int opt_norm(const OptPlan& P, const float* grad_scale,
     return 0;
 }
 
+// An AdamW step of few tensors: true if it was one (its return code in rc).
+template <int BITS>
+static bool adamw_few(const NndetOptTensor* t, int32_t n, const NndetAdamw* a, const OptScalars& S, const OptHyper& H, OptPlan& P, hipStream_t st, int* rc) {
+    OptTableArgs<BITS == 8 ? 6 : 4> A;
+    const bool clip = a->max_norm >= 0.0;
+    if (clip && a->norm_given) return false;
+    const int k = opt_few(t, n, clip ? OPT_FEW_TOTAL : INT64_MAX, S, P, A);
+    if (k < 0) return false;
+#define OPT_NORM(T) (k_opt_norm_few<T, false><<<1, OPT_FEW_WG, 0, st>>>(A, a->max_norm, a->norm))
+#define OPT_CALL(T) (k_adamw_few<T, BITS><<<n, OPT_WG, 0, st>>>(A, H, clip))
+    if (clip) NNDET_DISPATCH_DTYPE(k % 3, OPT_NORM);
+    NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL);
+#undef OPT_NORM
+#undef OPT_CALL
+    *rc = (int)hipGetLastError();
+    return true;
+}
+
 extern "C" int nndet_adamw_step(const NndetOptTensor* tensors, int32_t n, const NndetAdamw* a, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!a || !a->steps || !(a->beta1 >= 0.0 && a->beta1 < 1.0) || !(a->beta2 >= 0.0 && a->beta2 < 1.0) || !(a->eps >= 0.0)) return NNDET_EINVAL;
+    if (!a || !a->steps || !(a->beta1 >= 0.0 && a->beta1 < 1.0) || !(a->beta2 >= 0.0 && a->beta2 < 1.0) || !(a->eps == 0.0 || a->eps >= 0x1p-126)) return NNDET_EINVAL;
     if (a->max_norm != a->max_norm || (a->norm_given && (!a->norm || a->max_norm < 0.0))) return NNDET_EINVAL;
     hipStream_t st = as_stream(stream);
     const OptScalars S = {a->steps, a->lr_device, a->found_inf, a->grad_scale, a->lr, a->beta1, a->beta2};
+    const OptHyper H = {(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps};
     OptPlan P;
-    int rc = opt_begin(tensors, n, 7, S, OPT_NB, workspace, workspace_bytes, P, st);
+    int rc = opt_check(tensors, n, 7, workspace, workspace_bytes, P);
+    if (rc || adamw_few<32>(tensors, n, a, S, H, P, st, &rc) || adamw_few<8>(tensors, n, a, S, H, P, st, &rc)) return rc;
+    rc = opt_begin(tensors, n, S, OPT_NB, P, st);
     if (rc) return rc;
     if (a->max_norm >= 0.0) {
         rc = opt_norm<OPT_NB>(P, a->grad_scale, a->max_norm, a->norm, a->norm_given != 0, st);
         if (rc) return rc;
     }
-    const OptHyper H = {(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps};
     for (int k = 0; k < 6; ++k) {
         if (!P.tiles[k]) continue;
         const unsigned g = opt_grid(P.tiles[k], OPT_GRID);
@@ -623,7 +778,18 @@ extern "C" int nndet_grad_clip(const NndetOptTensor* tensors, int32_t n, double 
     hipStream_t st = as_stream(stream);
     const OptScalars S = {nullptr, nullptr, nullptr, nullptr, 0.0, 0.0, 0.0};
     OptPlan P;
-    int rc = opt_begin(tensors, n, 2, S, OPT_CLIP_NB, workspace, workspace_bytes, P, st);
+    int rc = opt_check(tensors, n, 2, workspace, workspace_bytes, P);
+    if (rc) return rc;
+    OptTableArgs<4> A;
+    const int few = opt_few(tensors, n, OPT_FEW_TOTAL, {nullptr, nullptr, nullptr, grad_scale, 0.0, 0.0, 0.0}, P, A);
+    if (few >= 0) {
+#define OPT_CALL(T) (k_opt_norm_few<T, true><<<1, OPT_FEW_WG, 0, st>>>(A, max_norm, norm_out))
+        NNDET_DISPATCH_DTYPE(few % 3, OPT_CALL);
+#undef OPT_CALL
+        LAUNCH_CHECK();
+        return 0;
+    }
+    rc = opt_begin(tensors, n, S, OPT_CLIP_NB, P, st);
     if (rc) return rc;
     rc = opt_norm<OPT_CLIP_NB>(P, grad_scale, max_norm, norm_out, false, st);
     if (rc || max_norm < 0.0) return rc;         // the norm alone
@@ -646,7 +812,17 @@ extern "C" int nndet_adam_state8(const NndetOptTensor* tensors, int32_t n, int32
     hipStream_t st = as_stream(stream);
     const OptScalars S = {nullptr, nullptr, nullptr, nullptr, 0.0, 0.0, 0.0};
     OptPlan P;
-    int rc = opt_begin(tensors, n, 7, S, OPT_NB, workspace, workspace_bytes, P, st);
+    int rc = opt_check(tensors, n, 7, workspace, workspace_bytes, P);
+    if (rc) return rc;
+    OptTableArgs<6> A;
+    const int few = opt_few(tensors, n, INT64_MAX, S, P, A);
+    if (few >= 0) {
+        if (write) k_opt_state8_few<true><<<n, OPT_WG, 0, st>>>(A);
+        else k_opt_state8_few<false><<<n, OPT_WG, 0, st>>>(A);
+        LAUNCH_CHECK();
+        return 0;
+    }
+    rc = opt_begin(tensors, n, S, OPT_NB, P, st);
     if (rc) return rc;
     const int k = NNDET_F32 + 3;
     if (!P.tiles[k]) return 0;

@@ -297,8 +297,8 @@ Rate = Union[float, torch.Tensor]
 def _hyper(lr, betas, eps, max_norm, total_norm, grad_scale, found_inf, steps, device):
     """The scalars of a step as the library takes them, checked, and the norm's tensor (None without clipping)."""
     b1, b2 = float(betas[0]), float(betas[1])
-    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
-        _refuse(f"betas {betas} in [0, 1) and eps {eps} >= 0 are wanted")
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and (eps == 0.0 or eps >= 2.0 ** -126)):
+        _refuse(f"betas {betas} in [0, 1) and an eps {eps} that is 0 or a normal fp32 number are wanted")
     if max_norm is not None and not max_norm >= 0.0:
         _refuse(f"max_norm {max_norm} >= 0 is wanted")
     if total_norm is not None and max_norm is None:
@@ -372,7 +372,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps: torch.Tensor, *, lr:
     params / grads: fp32, bf16 or fp16 tensors (any mixture) on one GPU, dense in memory; a gradient in another memory order is copied
     first, a gradient None leaves its tensor, moments and count as they are. exp_avgs / exp_avg_sqs: fp32, in the parameters' memory order.
     steps: int32 counts on the GPU, one a tensor. No two of the tensors may overlap. lr: a number, or one fp32 value on the GPU (a captured
-    step follows a schedule through it). weight_decay: a number, or one a tensor.
+    step follows a schedule through it). weight_decay: a number, or one a tensor. The step is computed in fp32; a 16-bit parameter is rounded
+    once, to nearest, so a change below half its unit is lost, as it is in torch.
     max_norm: the gradients are multiplied by min(1, max_norm / (norm + 1e-6)) on the way (they are not written), where norm is `total_norm`
     or else the 2-norm over all gradients of the call; the norm is returned, on the GPU. A norm that is not finite gives what it gives in
     torch's clipping: NaN. grad_scale: the gradients carry this loss scale and are divided by it, before the norm. found_inf: where it is

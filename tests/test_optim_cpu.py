@@ -49,7 +49,7 @@ def test_adamw_step_refuses_a_duplicate_parameter():
 
 @pytest.mark.parametrize("kw,match", [
     (dict(betas=(1.0, 0.9)), "betas"), (dict(betas=(0.9, -0.1)), "betas"), (dict(betas=(0.9, float("nan"))), "betas"), (dict(eps=-1e-8), "eps"),
-    (dict(eps=float("nan")), "eps"), (dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm"), (dict(total_norm=torch.zeros(())), "total_norm without"),
+    (dict(eps=float("nan")), "eps"), (dict(eps=1e-40), "eps"), (dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm"), (dict(total_norm=torch.zeros(())), "total_norm without"),
     (dict(weight_decay=[0.1]), "1 weight_decay for 2"), (dict(grad_scale=torch.zeros(2)), "grad_scale is one fp32"), (dict(grad_scale=2.0), "grad_scale is one fp32"),
     (dict(found_inf=torch.zeros((), dtype=torch.float64)), "found_inf is one fp32"), (dict(max_norm=1.0, total_norm=torch.zeros(3)), "total_norm is one fp32"),
     (dict(lr=torch.zeros(2)), "lr is one fp32"), (dict(), "no CPU path"),
@@ -121,9 +121,9 @@ def test_the_library_checks_its_arguments():
     one = (L.NndetOptTensor * 1)()
     t = one[0]
     a = L.NndetAdamw(1e-3, 0.9, 0.999, 1e-8, -1.0)
-    ws = (C.c_char * (1 << 16))()
+    ws = (C.c_char * (1 << 18))()
     at = (C.addressof(ws) + 15) // 16 * 16
-    size = 1 << 15
+    size = 1 << 17
 
     def step(n=1, ws=at, size=size, args=a, tensors=one):
         return lib.nndet_adamw_step(tensors, n, C.byref(args) if args is not None else None, ws, size, None)
@@ -134,12 +134,12 @@ def test_the_library_checks_its_arguments():
     a.steps = 16
     assert step(n=-1) == -1 and step(tensors=None) == -1 and step(ws=None) == -1 and step(ws=at + 4) == -1 and step(size=64) == -2
     for field, bad in (("dtype", 3), ("dtype", -1), ("state_bits", 16), ("numel", -1), ("numel", 1 << 40), ("slot", -1), ("slot", 1 << 24), ("param", 0),
-                       ("grad", 0), ("exp_avg", 0), ("exp_avg_sq", 0), ("state_bits", 8)):
+                       ("grad", 0), ("grad", 1 << 48), ("exp_avg", 0), ("exp_avg_sq", 0), ("state_bits", 8)):
         old = getattr(t, field)
         setattr(t, field, bad)
         assert step() == -1, field
         setattr(t, field, old)
-    for field, bad in (("beta1", 1.0), ("beta2", -0.5), ("beta2", float("nan")), ("eps", -1.0), ("max_norm", float("nan")), ("norm_given", 1)):
+    for field, bad in (("beta1", 1.0), ("beta2", -0.5), ("beta2", float("nan")), ("eps", -1.0), ("eps", 1e-40), ("max_norm", float("nan")), ("norm_given", 1)):
         old = getattr(a, field)
         setattr(a, field, bad)
         assert step() == -1, field
