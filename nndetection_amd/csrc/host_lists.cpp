@@ -7,7 +7,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/core/TensorBody.h>
 
-#include <algorithm>
+#include <cstring>
 #include <vector>
 
 #include "../../include/nndet_amd.h"
@@ -32,7 +32,7 @@ const c10::TensorImpl* plain(const at::TensorBase& t, c10::DeviceIndex device) {
     if (!t.defined()) return nullptr;
     const c10::TensorImpl* x = t.unsafeGetTensorImpl();
     if (x->layout() != c10::kStrided || x->is_python_dispatch() || x->device() != c10::Device(c10::kCUDA, device)) return nullptr;
-    if (!x->is_non_overlapping_and_dense() || (x->numel() && !x->data())) return nullptr;
+    if (!(x->is_contiguous() || x->is_non_overlapping_and_dense()) || (x->numel() && !x->data())) return nullptr;
     return x;
 }
 const c10::TensorImpl* plain(PyObject* o, c10::DeviceIndex device) {
@@ -54,8 +54,25 @@ int type_of(const c10::TensorImpl* x) {
 }
 bool is(const c10::TensorImpl* x, c10::ScalarType t) { return c10::typeMetaToScalarType(x->dtype()) == t; }
 
-// pack(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, root_scales, weight_decay, bits, device,
-//      both) -> (structs, n) or None
+struct Addresses {                                   // a set of addresses: open addressing, at most half full
+    std::vector<const void*> slot;
+    size_t mask;
+    explicit Addresses(size_t n) {
+        size_t size = 16;
+        while (size < 2 * n) size *= 2;
+        slot.assign(size, nullptr);
+        mask = size - 1;
+    }
+    bool add(const void* p) {                        // false if it is there already
+        for (size_t i = ((uintptr_t)p >> 4) * 0x9E3779B97F4A7C15ull >> 32 & mask;; i = (i + 1) & mask) {
+            if (slot[i] == p) return false;
+            if (!slot[i]) { slot[i] = p; return true; }
+        }
+    }
+};
+
+// pack(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, root_scales, weight_decay, bits, device, both)
+//   -> (structs, n) or None
 //   params None: grads alone. grads None: params[i].grad. A gradient that is None leaves its tensor out (slot = place in the list).
 //   exp_avgs None: no moments. bits: 32, 8, or 0 for either, by the type of exp_avgs[i]. weight_decay: a number or a list.
 //   both: grads are written too.
@@ -78,8 +95,7 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         PyObject* out = PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(NndetOptTensor));
         if (!out) return nullptr;
         NndetOptTensor* t = reinterpret_cast<NndetOptTensor*>(PyBytes_AS_STRING(out));
-        std::vector<void*> at;
-        at.reserve(4 * n);
+        Addresses seen((p.seq ? 1 + (both != 0) : 1) * n + (m.seq ? 2 * n : 0));
         Py_ssize_t k = 0;
         for (Py_ssize_t i = 0; i < n; ++i) {
             const c10::TensorImpl *px = nullptr, *gx = nullptr;
@@ -130,14 +146,11 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                 }
             }
             if (e.numel) {                           // what a call writes: no address twice
-                at.push_back(e.param ? e.param : e.grad);
-                if (px && both) at.push_back(e.grad);
-                if (m.seq) { at.push_back(e.exp_avg); at.push_back(e.exp_avg_sq); }
+                if (!seen.add(px ? e.param : e.grad) || (px && both && !seen.add(e.grad))) goto other;
+                if (m.seq && (!seen.add(e.exp_avg) || !seen.add(e.exp_avg_sq))) goto other;
             }
             ++k;
         }
-        std::sort(at.begin(), at.end());
-        if (std::adjacent_find(at.begin(), at.end()) != at.end()) goto other;
         if (k != n && _PyBytes_Resize(&out, k * (Py_ssize_t)sizeof(NndetOptTensor)) < 0) return nullptr;
         return Py_BuildValue("Nn", out, k);
     other:

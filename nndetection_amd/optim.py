@@ -317,8 +317,16 @@ def _hyper(lr, betas, eps, max_norm, total_norm, grad_scale, found_inf, steps, d
     return a, norm
 
 
+def _listed(*args):
+    """Each argument as a list or tuple (None stays None)."""
+    return [x if x is None or isinstance(x, (list, tuple)) else list(x) for x in args]
+
+
 def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight_decay, max_norm, total_norm, grad_scale, found_inf):
+    params, grads, m, v, ms, rs = _listed(params, grads, m, v, ms, rs)
     n = len(params)
+    if bits == 8:
+        _check_lengths(n, exp_avg_scale=ms, root_scale=rs)
     _check_lengths(n, grads=grads, exp_avgs=m, exp_avg_sqs=v)
     if not isinstance(steps, torch.Tensor) or steps.dtype != torch.int32 or steps.dim() != 1 or not steps.is_contiguous() or steps.numel() < n:
         _refuse(f"steps is one int32 count a tensor ({n}), contiguous")
@@ -390,7 +398,6 @@ def adamw8_step(params, grads, state: AdamState8, steps: torch.Tensor, *, lr: Ra
     that keeps its expected value (by bits that follow from the element's index and its step count: the same step gives the same state).
     A gradient that is not finite makes the moments of its whole block NaN; `found_inf` keeps it out."""
     m, ms, v, rs = state
-    _check_lengths(len(params), exp_avg_scale=ms, root_scale=rs)
     return _adamw_call(params, grads, m, v, ms, rs, 8, steps, lr, betas, eps, weight_decay, max_norm, total_norm, grad_scale, found_inf)
 
 
@@ -450,6 +457,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0) -> torc
 
 
 def _state8_call(state: AdamState8, exp_avgs, exp_avg_sqs, write: int) -> None:
+    exp_avgs, exp_avg_sqs, *state = _listed(exp_avgs, exp_avg_sqs, *state)
+    state = AdamState8(*state)
     n = len(exp_avgs)
     _check_lengths(n, exp_avg_sqs=exp_avg_sqs, exp_avg=state.exp_avg, exp_avg_scale=state.exp_avg_scale, root=state.root, root_scale=state.root_scale)
     if n == 0:
@@ -502,9 +511,13 @@ class AdamW:
             _refuse(f"state_bits {state_bits}: 32 or 8")
         if max_norm is not None and not max_norm >= 0.0:
             _refuse(f"max_norm {max_norm} >= 0 is wanted")
-        groups = list(param_groups)
+        groups = [param_groups] if isinstance(param_groups, torch.Tensor) else list(param_groups)
         if groups and not isinstance(groups[0], dict):
             groups = [{"params": groups}]
+        for g in [{"weight_decay": weight_decay, "betas": betas, "eps": eps}, *groups]:
+            wd, (b1, b2), e = g.get("weight_decay", 0.0), g.get("betas", betas), g.get("eps", eps)
+            if not (wd >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and (e == 0.0 or e >= 2.0 ** -126)):
+                _refuse(f"weight_decay {wd} >= 0, betas {(b1, b2)} in [0, 1) and an eps {e} that is 0 or a normal fp32 number are wanted")
         self.defaults = {"lr": float(lr), "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay}
         self.param_groups = []
         for g in groups:
@@ -553,7 +566,7 @@ class AdamW:
         self._state[p] = st
         for ts, k in zip(self._lists, ("exp_avg", "root" if bits == 8 else "exp_avg_sq", "exp_avg_scale", "root_scale")):
             ts[self._slot[p]] = st.get(k)
-        self._fixed[p] = (*at, p.numel(), self._slot[p] | _KIND[p.dtype] | (bits << 48), p.stride(), p.device)
+        self._fixed[p] = (*at, p.numel(), self._slot[p] | (bits << 48), p.stride(), p.device)
 
     @torch.no_grad()
     def step(self) -> None:
@@ -586,8 +599,8 @@ class AdamW:
                 m, v, ms, rs, numel, tail, stride, device = fixed
                 if p.device != device or p.numel() != numel or p.stride() != stride:
                     _refuse(f"a parameter of shape {tuple(p.shape)} on {p.device} was moved or changed its size after its state was made")
-                if gr.stride() != stride or gr.is_sparse:
-                    gr = _grads_like([p], [gr])[0]
+                tail |= _kinds([p])[0]               # (its type may have changed: the moments are fp32 or 8 bits whatever it is)
+                gr = _grads_like([p], [gr])[0]
                 c = calls.get((device, key))
                 if c is None:
                     c = calls[(device, key)] = ([], [], [], g)
@@ -604,6 +617,7 @@ class AdamW:
                 per.setdefault(device, []).extend(c[2])
             norms = [grad_norm(gs, on(scale, device)) for device, gs in per.items()]
             total = norms[0] if len(norms) == 1 else torch.stack([x.to(norms[0].device, torch.float64) for x in norms]).square().sum().sqrt().float()
+        _check_distinct("the parameters", [p for c in calls.values() for p in c[1]])
         for (device, _), (words, ps, _, g) in calls.items():
             counts = self._counts(device)
             a, self.grad_norm = _hyper(g["lr"], g["betas"], g["eps"], self.max_norm, on(total, device), on(scale, device), on(found, device),

@@ -152,9 +152,11 @@ def test_the_library_checks_its_arguments():
 
 def test_optimizer_refuses():
     p = [torch.nn.Parameter(torch.zeros(5)), torch.nn.Parameter(torch.zeros(3))]
-    for kw, match in ((dict(state_bits=16), "state_bits"), (dict(max_norm=-1.0), "max_norm")):
+    for kw, match in ((dict(state_bits=16), "state_bits"), (dict(max_norm=-1.0), "max_norm"), (dict(weight_decay=-0.1), "weight_decay"), (dict(betas=(0.9, 1.0)), "betas"),
+                      (dict(eps=float("nan")), "eps")):
         refused(match, lambda: O.AdamW(p, **kw))
     refused("twice", lambda: O.AdamW([{"params": p}, {"params": p[:1]}]))
+    refused("eps", lambda: O.AdamW([{"params": p, "eps": 1e-42}]))
     refused("amsgrad", lambda: O.AdamW([{"params": p, "amsgrad": True}]))
     refused("float64", lambda: O.AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float64))]))
     opt = O.AdamW(p)

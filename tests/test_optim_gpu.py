@@ -552,6 +552,52 @@ def test_training_loop_with_scaler_clipping_and_schedule(bits):
     assert all(torch.equal(x, y) for x, y in zip(*grads))
 
 
+def test_parameters_that_change_their_type_or_share_memory():
+    """A module may be cast after its state was made (the moments stay as they are), gradients may lie in another order than their parameters, and two
+    parameters on one piece of memory are refused."""
+    for strided in (False, True):
+        g = gen(60)
+        p = torch.nn.Parameter(torch.randn(40, 300, generator=g, device=DEV))
+        opt = O.AdamW(p, lr=1e-2, weight_decay=0.0)
+        fresh = lambda: torch.randn(300, 40, generator=g, device=DEV).t() if strided else torch.randn(40, 300, generator=g, device=DEV)  # noqa: E731
+        p.grad = fresh()
+        opt.step()
+        st = opt.state_dict()["state"][0]
+        m, v = st["exp_avg"].clone(), st["exp_avg_sq"].clone()
+        p.grad = None
+        p.data = p.data.bfloat16()
+        p.grad = fresh().bfloat16()
+        wp, wm, wv = formula(p.detach(), p.grad, m, v, 2, 1e-2, 0.9, 0.999, 1e-8, 0.0)
+        opt.step()
+        within(p.detach(), *wp, torch.bfloat16)
+        within(st["exp_avg"], *wm)
+        within(st["exp_avg_sq"], *wv)
+        p.data = p.data[:20].clone()
+        p.grad = None
+        p.grad = torch.zeros_like(p)
+        with pytest.raises(L.NndetError, match="changed its size"):
+            opt.step()
+    base = torch.zeros(100, device=DEV)
+    ps = [torch.nn.Parameter(base), torch.nn.Parameter(base.view(10, 10))]
+    opt = O.AdamW(ps)
+    for q in ps:
+        q.grad = torch.ones_like(q)
+    for _ in range(2):
+        with pytest.raises(L.NndetError, match="twice"):
+            opt.step()
+    assert not base.any()
+
+
+def test_any_iterable_is_a_list():
+    x = make([700, 33], torch.float32, seed=61)
+    y = make([700, 33], torch.float32, seed=61)
+    steps, steps2 = (torch.zeros(2, dtype=torch.int32, device=DEV) for _ in range(2))
+    O.adamw_step(x["p"], x["g"], x["m"], x["v"], steps, lr=0.1)
+    O.adamw_step(iter(y["p"]), tuple(y["g"]), dict(enumerate(y["m"])).values(), (t for t in y["v"]), steps2, lr=0.1)
+    assert all(torch.equal(a, b) for k in "pmv" for a, b in zip(x[k], y[k])) and torch.equal(steps, steps2)
+    assert all(p._version > 0 for p in y["p"])
+
+
 @pytest.mark.parametrize("have,want", [(32, 8), (8, 32), (8, 8)])
 def test_checkpoints_convert(have, want):
     net = network(2)
