@@ -2,7 +2,7 @@
 // conversion between fp32 and 8-bit moments.
 //
 // A call takes n tensors of any sizes. k_opt_table copies their addresses out of the kernel arguments into a table in the workspace (64 B
-// a tensor, up to 99 of them a launch, so that every later kernel is ONE launch whatever n is), advances the step counts and works out what
+// a tensor, up to 99 of them a launch (166 gradients), so that every later kernel is ONE launch whatever n is), advances the step counts and works out what
 // is the same for a whole tensor. Then one launch per storage kind (type of the parameters x bits of the moments) has a workgroup for each
 // tile of 2048 consecutive elements of a tensor; no tile spans two tensors. A wave owns blocks of 256 consecutive elements, which are also
 // the blocks that share a scale of the 8-bit moments: the maximum never leaves the wave. Calls of few small tensors skip the table.
@@ -37,7 +37,8 @@ static constexpr int OPT_BLOCK = 256;            // elements of a wave's block =
 static constexpr int OPT_NB = 2, OPT_CLIP_NB = 4;
 // One workgroup a tile up to this many (a grid is limited to 2^32 threads). 2048 workgroups that walk over the tiles instead were 15 - 20 % slower.
 static constexpr int OPT_GRID = 1 << 20;
-static constexpr int OPT_PARTIALS = 1024;        // workgroups (and fp64 partial sums) of the norm per storage kind
+static constexpr int OPT_PARTIALS = 2048;        // workgroups (and fp64 partial sums) of the norm per storage kind (1024: 1 - 2 % slower)
+static constexpr int OPT_NORM_WG = 1024;         // threads of the workgroup that adds them up
 // The kernels for few small tensors take one workgroup a tensor, and one for the norm of all. Against the table's kernels (1 to 60 tensors, us of
 // GPU time / of a call with its host time): 4000 elements 5.4 / 10.4 against 6.5 / 13.7, 8000 elements 7.4 against 6.3; norm and clipping of 60 k
 // elements in all 6.7 / 12.5 against 8.8 / 20.8, of 120 k 9.4 against 8.9.
@@ -53,17 +54,17 @@ static_assert(sizeof(OptEntry) == 64, "four 16-byte stores");
 struct OptCoef { float size, unbias, decay; uint32_t t; };
 struct OptHead { float factor; int32_t skip; int32_t pad[14]; };
 
-// A tensor in the kernel arguments: its PTRS addresses (48 bits each; 4: param, grad, moments, 6: and the scales), numel below 2^40, slot.
+// A tensor in the kernel arguments: its PTRS addresses (48 bits each; 1: grad, 4: param, grad, moments, 6: and the scales), numel below 2^40, slot.
 template <int PTRS> struct OptArg { uint32_t lo[PTRS]; uint16_t hi[PTRS]; uint32_t numel_lo, numel_hi_slot; float wd; uint32_t tile0; };
 template <int PTRS> struct OptTableArgs {
-    static constexpr int MOST = PTRS == 4 ? 99 : 76;     // tensors a launch: what 4 KB of kernel arguments hold
+    static constexpr int MOST = PTRS == 1 ? 166 : PTRS == 4 ? 99 : 76;     // tensors a launch: what 4 KB of kernel arguments hold
     OptHead* head; OptEntry* entry; OptCoef* coef; uint32_t* tile0; int32_t* steps;
     const float* lr_ptr; const float* found_inf; const float* grad_scale;
     double lr, log2_b1, log2_b2;
     int32_t n, first;                                    // tensors of this launch; first: it also writes the head
     OptArg<PTRS> a[MOST];
 };
-static_assert(sizeof(OptTableArgs<4>) <= 4096 && sizeof(OptTableArgs<6>) <= 4096, "kernel arguments are limited to 4 KB");
+static_assert(sizeof(OptTableArgs<1>) <= 4096 && sizeof(OptTableArgs<4>) <= 4096 && sizeof(OptTableArgs<6>) <= 4096, "kernel arguments are limited to 4 KB");
 
 // After 16-byte stores, with all arithmetic before them (a sched_barrier): nothing may overwrite a store's data registers in its next slots
 // (tools/scan_store_hazard.py).
@@ -75,7 +76,7 @@ __device__ __forceinline__ void opt_stored() {
 template <int PTRS> __device__ __forceinline__ OptEntry opt_entry(const OptArg<PTRS>& a) {
     uint64_t at[6] = {0, 0, 0, 0, 0, 0};
 #pragma unroll
-    for (int k = 0; k < PTRS; ++k) at[k] = a.lo[k] | (uint64_t)a.hi[k] << 32;
+    for (int k = 0; k < PTRS; ++k) at[PTRS == 1 ? 1 : k] = a.lo[k] | (uint64_t)a.hi[k] << 32;
     return {(void*)at[0], (const void*)at[1], (void*)at[2], (void*)at[3], (float*)at[4], (float*)at[5],
             (int64_t)(a.numel_lo | (uint64_t)(a.numel_hi_slot & 0xffu) << 32), 0};
 }
@@ -92,7 +93,7 @@ template <int PTRS> __device__ __forceinline__ bool opt_skip(const OptTableArgs<
 template <int PTRS> __device__ __forceinline__ float opt_factor(const OptTableArgs<PTRS>& A) { return A.grad_scale ? (float)(1.0 / (double)*A.grad_scale) : 1.0f; }
 
 template <int PTRS>
-__global__ __launch_bounds__(128) void k_opt_table(const OptTableArgs<PTRS> A) {
+__global__ __launch_bounds__(192) void k_opt_table(const OptTableArgs<PTRS> A) {
     const int i = threadIdx.x;
     const bool skip = opt_skip(A);
     if (A.first && i == 0) {
@@ -239,11 +240,11 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t x) {          // DPP: 
     return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 // scale of a block from its values: max |x| / 448, 0 where that is below 2^-110 (1 / scale stays finite). Magnitudes are compared as
-// integers, so a NaN (an inf) is the largest and makes the scale NaN (inf): the block then reads back as NaN.
-__device__ __forceinline__ float opt_scale(const float* x) {
+// integers, so a NaN (an inf) is the largest and makes the scale NaN (inf): the block then reads back as NaN. ROOT: no signs.
+template <bool ROOT> __device__ __forceinline__ float opt_scale(const float* x) {
     uint32_t a = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) { const uint32_t b = __float_as_uint(x[k]) & 0x7fffffffu; a = b > a ? b : a; }
+    for (int k = 0; k < 4; ++k) a = max(a, ROOT ? __float_as_uint(x[k]) : __float_as_uint(x[k]) & 0x7fffffffu);
     const float s = __uint_as_float(wave_max_u32(a)) * (float)(1.0 / 448.0);
     return s < 0x1p-110f ? 0.0f : s;
 }
@@ -251,8 +252,22 @@ __device__ __forceinline__ void opt_decode(uint32_t c, float s, float* x) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
     x[0] = lo[0] * s; x[1] = lo[1] * s; x[2] = hi[0] * s; x[3] = hi[1] * s;
 }
+// Square root and quotient of the 8-bit step, which with the IEEE sequences kept its vector units busy for 73 % (19.0 M elements) to 94 % (295 M) of
+// the time: 85 instructions an element, now 65. 19 and 13 issue slots for those sequences, 11 and 8 for these: 60.5 -> 57.7 us at 19.0 M, no change at
+// 295 M; with 16-bit parameters (10 B an element) the vector units stay the bound: 60 M elements of fp16 146 -> 136 us (4.4 TB/s), of bf16 128 -> 124.
+// One residual step behind the hardware's reciprocal (root): correctly rounded but for about one value in 2^22.
+__device__ __forceinline__ float opt_root(float v) {
+    const float y = __builtin_amdgcn_rsqf(v), s = v * y;
+    const float r = fmaf(fmaf(-s, s, v), 0.5f * y, s);
+    return __builtin_amdgcn_classf(v, 0x100) ? r : v * 0x1p-24f;         // not a positive normal number: 0, inf and NaN are their own roots, denormals go to 0
+}
+__device__ __forceinline__ float opt_quotient(float m, float d) {       // d is not a denormal: roots are 0 or above 2^-63, eps is 0 or normal, scales 0 or above 2^-110
+    const float y = __builtin_amdgcn_rcpf(d), q = m * y;
+    return __builtin_amdgcn_div_fixupf(fmaf(fmaf(-d, q, m), y, q), d, m);
+}
+
 // 1 / scale, 0 for a block of zeros (whose codes are then 0)
-__device__ __forceinline__ float opt_inverse(float s) { return s == 0.0f ? 0.0f : 1.0f / s; }
+__device__ __forceinline__ float opt_inverse(float s) { return s == 0.0f ? 0.0f : opt_quotient(1.0f, s); }
 __device__ __forceinline__ uint32_t opt_encode(const float* x, float s, bool root) {      // to nearest even
     const float inv = opt_inverse(s);
     float y[4];
@@ -287,19 +302,6 @@ template <bool FULL> __device__ __forceinline__ uint32_t opt_encode_root(const f
         c |= min(max(q, least), 0x7eu) << (8 * k);
     }
     return c;
-}
-
-// Square root and quotient of the 8-bit step, which with the IEEE sequences kept its vector units busy for 73 % (19.0 M elements) to 94 % (295 M) of
-// the time: 85 instructions an element. 19 and 13 issue slots for those sequences, 11 and 8 for these: 60.5 -> 58.3 us at 19.0 M, no change at 295 M.
-// One residual step behind the hardware's reciprocal (root): correctly rounded but for about one value in 2^22.
-__device__ __forceinline__ float opt_root(float v) {
-    const float y = __builtin_amdgcn_rsqf(v), s = v * y;
-    const float r = fmaf(fmaf(-s, s, v), 0.5f * y, s);
-    return __builtin_amdgcn_classf(v, 0x100) ? r : v * 0x1p-24f;         // not a positive normal number: 0, inf and NaN are their own roots, denormals go to 0
-}
-__device__ __forceinline__ float opt_quotient(float m, float d) {       // d is not a denormal: the root is 0 or above 2^-63, and so is eps
-    const float y = __builtin_amdgcn_rcpf(d), q = m * y;
-    return __builtin_amdgcn_div_fixupf(fmaf(fmaf(-d, q, m), y, q), d, m);
 }
 
 // Runs f over the blocks of the walk's tiles: f(OptWhole<U>, base, 256) on U whole blocks of an aligned tensor (4 * OPT_BLOCK apart), f(OptPart, base,
@@ -373,7 +375,7 @@ __device__ __forceinline__ void adamw_block(const OptEntry& e, int64_t base, int
                 for (int k = 0; k < 4; ++k)
                     if (lane + 64 * k >= rem) m[u][k] = r[k] = 0.0f;
             }
-            const float nm = opt_scale(m[u]), nr = opt_scale(r);
+            const float nm = opt_scale<false>(m[u]), nr = opt_scale<true>(r);
             cm[u] = opt_encode(m[u], nm, false);
             cv[u] = opt_encode_root<FULL>(r, nr, at + (FULL ? 4 * lane : lane), c.t);
             sm[u] = nm; sr[u] = nr;
@@ -437,16 +439,16 @@ __device__ __forceinline__ float opt_clip(float norm, const float* grad_scale, d
 
 // The norm (count < 0: given at norm_at) and the factor. One workgroup, a launch of its own: 4 us. Finishing in the last workgroup of k_opt_sumsq
 // instead (a ticket) was no faster: 1024 tickets on one address take 6 us, and with 256 larger workgroups the sums themselves take 3 us more.
-__global__ __launch_bounds__(OPT_PARTIALS) void k_opt_norm(const double* partial, int count, const float* grad_scale, double max_norm, float* norm_at, OptHead* head) {
-    __shared__ double part[OPT_PARTIALS / 64];
+__global__ __launch_bounds__(OPT_NORM_WG) void k_opt_norm(const double* partial, int count, const float* grad_scale, double max_norm, float* norm_at, OptHead* head) {
+    __shared__ double part[OPT_NORM_WG / 64];
     double s = 0.0;
-    for (int i = threadIdx.x; i < count; i += OPT_PARTIALS) s += partial[i];
+    for (int i = threadIdx.x; i < count; i += OPT_NORM_WG) s += partial[i];
     s = wave_sum_f64(s);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         double sum = 0.0;
-        for (int k = 0; k < OPT_PARTIALS / 64; ++k) sum += part[k];
+        for (int k = 0; k < OPT_NORM_WG / 64; ++k) sum += part[k];
         const float norm = count < 0 ? *norm_at : opt_norm_of(sum, grad_scale);
         head->factor = opt_clip(norm, grad_scale, max_norm);
         if (norm_at && count >= 0) *norm_at = norm;
@@ -485,7 +487,7 @@ template <bool FULL, bool WRITE> __device__ __forceinline__ void opt_state8_bloc
         opt_load<FULL, true>(opt_at<float>(e.g, base), lane, rem, v);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = sqrtf(v[k]);
-        const float sm = opt_scale(m), sr = opt_scale(v);
+        const float sm = opt_scale<false>(m), sr = opt_scale<true>(v);
         opt_store_codes<FULL>(opt_at<uint8_t>(e.m, base), lane, rem, opt_encode(m, sm, false));
         opt_store_codes<FULL>(opt_at<uint8_t>(e.v, base), lane, rem, opt_encode(v, sr, true));
         if (lane == 0) { *opt_at<float>(e.ms, block) = sm; *opt_at<float>(e.rs, block) = sr; }
@@ -611,7 +613,8 @@ template <int PTRS> static void opt_scalars(const OptScalars& S, OptHead* head, 
 template <int PTRS> static void opt_arg(const NndetOptTensor& t, uint32_t tile0, OptArg<PTRS>& a) {
     const uint64_t p[6] = {(uint64_t)t.param, (uint64_t)t.grad, (uint64_t)t.exp_avg, (uint64_t)t.exp_avg_sq, (uint64_t)t.exp_avg_scale, (uint64_t)t.root_scale};
     for (int q = 0; q < PTRS; ++q) {
-        a.lo[q] = (uint32_t)p[q]; a.hi[q] = (uint16_t)(p[q] >> 32);
+        const uint64_t at = p[PTRS == 1 ? 1 : q];
+        a.lo[q] = (uint32_t)at; a.hi[q] = (uint16_t)(at >> 32);
     }
     a.numel_lo = (uint32_t)t.numel; a.numel_hi_slot = (uint32_t)(t.numel >> 32) | (uint32_t)t.slot << 8;
     a.wd = (float)t.weight_decay;
@@ -638,7 +641,7 @@ static int opt_table(const NndetOptTensor* t, int32_t n, const OptScalars& S, in
             const bool end = i == n && k == k0 + 2;
             if (A.n == OptTableArgs<PTRS>::MOST || (end && (A.n || A.first))) {
                 A.entry = P.entry + at - A.n; A.coef = P.coef + at - A.n; A.tile0 = P.tile0 + at - A.n;
-                k_opt_table<PTRS><<<1, 128, 0, st>>>(A);
+                k_opt_table<PTRS><<<1, 192, 0, st>>>(A);
                 LAUNCH_CHECK();
                 A.n = 0; A.first = 0;
             }
@@ -674,12 +677,12 @@ static int opt_check(const NndetOptTensor* t, int32_t n, int need, void* ws, siz
 }
 
 // Writes the table.
-static int opt_begin(const NndetOptTensor* t, int32_t n, const OptScalars& S, int nb, OptPlan& P, hipStream_t st) {
+static int opt_begin(const NndetOptTensor* t, int32_t n, const OptScalars& S, int nb, OptPlan& P, hipStream_t st, bool grads_alone = false) {
     bool any8 = false, any32 = n == 0;
     for (int i = 0; i < n; ++i) (t[i].state_bits == 8 ? any8 : any32) = true;
     P.first[0] = 0;
     int rc = 0;
-    if (any32) rc = opt_table<4>(t, n, S, nb, 0, true, P, st);
+    if (any32) rc = grads_alone ? opt_table<1>(t, n, S, nb, 0, true, P, st) : opt_table<4>(t, n, S, nb, 0, true, P, st);
     else for (int k = 0; k < 4; ++k) { P.first[k] = 0; if (k < 3) P.tiles[k] = 0; }
     if (rc) return rc;
     if (any8) return opt_table<6>(t, n, S, nb, 3, !any32, P, st);
@@ -718,7 +721,7 @@ template <int NB> static int opt_norm(const OptPlan& P, const float* grad_scale,
         LAUNCH_CHECK();
         count += (int)g;
     }
-    k_opt_norm<<<1, OPT_PARTIALS, 0, st>>>(P.partial, given ? -1 : count, grad_scale, max_norm, norm, P.head);
+    k_opt_norm<<<1, OPT_NORM_WG, 0, st>>>(P.partial, given ? -1 : count, grad_scale, max_norm, norm, P.head);
     LAUNCH_CHECK();
     return 0;
 }
@@ -780,7 +783,9 @@ extern "C" int nndet_grad_clip(const NndetOptTensor* tensors, int32_t n, double 
     OptPlan P;
     int rc = opt_check(tensors, n, 2, workspace, workspace_bytes, P);
     if (rc) return rc;
-    OptTableArgs<4> A;
+    for (int i = 0; i < n; ++i)
+        if (tensors[i].state_bits != 32) return NNDET_EINVAL;
+    OptTableArgs<1> A;
     const int few = opt_few(tensors, n, OPT_FEW_TOTAL, {nullptr, nullptr, nullptr, grad_scale, 0.0, 0.0, 0.0}, P, A);
     if (few >= 0) {
 #define OPT_CALL(T) (k_opt_norm_few<T, true><<<1, OPT_FEW_WG, 0, st>>>(A, max_norm, norm_out))
@@ -789,7 +794,7 @@ extern "C" int nndet_grad_clip(const NndetOptTensor* tensors, int32_t n, double 
         LAUNCH_CHECK();
         return 0;
     }
-    rc = opt_begin(tensors, n, S, OPT_CLIP_NB, P, st);
+    rc = opt_begin(tensors, n, S, OPT_CLIP_NB, P, st, true);
     if (rc) return rc;
     rc = opt_norm<OPT_CLIP_NB>(P, grad_scale, max_norm, norm_out, false, st);
     if (rc || max_norm < 0.0) return rc;         // the norm alone
