@@ -52,7 +52,7 @@ int norm_finalize_run(const double* stats, int N, int c, int c_p, int groups, in
 // sees bit-identical activations to one that reads the materialised tensor.
 template <typename T> struct AffinePiece {       // the 16-bit storage types (bf16_t, f16_t: both sign-magnitude)
     static constexpr int E = 8;
-    // 20 VALU ops per piece: 8 unpack, 4 v_pk_fma_f32, 4 v_cvt_pk_bf16_f32, 4 v_pk_max_i16 (ReLU on the packed pair: a
+    // 24 VALU ops per piece: 8 unpack, 8 v_fma_f32, 4 v_cvt_pk_bf16_f32, 4 v_pk_max_i16 (ReLU on the packed pair: a
     // negative bf16 / fp16 -- incl. -0 -- is a negative int16; rounding is monotone, so relu(round(x)) == round(relu(x)))
     __device__ static __forceinline__ u32x4 apply(const u32x4 v, const float* sc, const float* sh, int relu) {
         typedef short s16x2 __attribute__((ext_vector_type(2)));

@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256, 1) void k_ig3s(const Ig3sArgs A) {
     __amdgpu_buffer_rsrc_t trs = qrs;                      // xn at the origin of the tile being transformed
     uint32_t tmask = 0;
     int t_n = -1, ss_n = -1;
-    f32x2_t scp[4], shp[4];                                // (pairs: the operands of v_pk_fma_f32)
+    f32x2_t scp[4], shp[4];                                // (pairs, as AffinePiece takes them)
     const uint32_t floor2 = A.ss_relu ? 0u : 0x80008000u;  // v_pk_max_i16 against (0, 0) = ReLU on the packed pair (AffinePiece); against INT16_MIN = identity
     u32x4 tv = {0, 0, 0, 0}, tr = {0, 0, 0, 0};
     auto take_t = [&]() {                                  // the decoded tile becomes the one to transform

@@ -124,8 +124,8 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             e.dtype = (int16_t)type;
             e.state_bits = 32;
             if (listed) {
-                e.weight_decay = PyFloat_AsDouble(wd[i]);
-                if (e.weight_decay == -1.0 && PyErr_Occurred()) { PyErr_Clear(); goto other; }
+                if (!PyFloat_Check(wd[i])) goto other;   // (no Python code runs here that could change the lists)
+                e.weight_decay = PyFloat_AS_DOUBLE(wd[i]);
             } else {
                 e.weight_decay = one_wd;
             }

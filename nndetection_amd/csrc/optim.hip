@@ -21,8 +21,8 @@
 // t alone (opt_mix), so a step is reproducible. An r that is not zero is not stored as zero: m / (0 + eps) would be a step of any size.
 //
 // Bound: HBM. Every input is read once and every output written once, 28 B an element with fp32 moments and 16.06 B with 8-bit ones (fp32
-// parameters). Measured (k_adamw alone, fp32 parameters): 295.5 M elements 1.44 ms = 5.7 TB/s and 0.76 ms = 6.2 TB/s (a large copy on the
-// same card: 4.7 - 5.0, a large in-place product 5.9 TB/s); 19.0 M elements 77 us = 6.9 TB/s and 50 us = 6.1 TB/s (part of it stays in the
+// parameters). Measured (k_adamw alone, fp32 parameters): 295.5 M elements 1.46 ms = 5.7 TB/s and 0.76 ms = 6.3 TB/s (a large copy on the
+// same card: 4.7 - 5.0, a large in-place product 5.9 TB/s); 19.0 M elements 78 us = 6.8 TB/s and 52 us = 5.8 TB/s (part of it stays in the
 // 256 MB cache between steps).
 #include "common.h"
 #include <math.h>

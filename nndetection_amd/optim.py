@@ -281,8 +281,8 @@ def _grads_like(params, grads) -> list:
     """Gradients in the parameters' memory order (a copy where they are not)."""
     out = []
     for i, (p, g) in enumerate(zip(params, grads)):
-        if g.is_sparse or g.shape != p.shape:
-            _refuse(f"grads[{i}] is {'sparse' if g.is_sparse else 'of shape %s' % (tuple(g.shape),)}, the parameter is dense {tuple(p.shape)}")
+        if g.layout != torch.strided or g.shape != p.shape:
+            _refuse(f"grads[{i}] is {'sparse' if g.layout != torch.strided else 'of shape %s' % (tuple(g.shape),)}, the parameter is dense {tuple(p.shape)}")
         if g.dtype != p.dtype or g.device != p.device:
             _refuse(f"grads[{i}] is {g.dtype} on {g.device}, the parameter {p.dtype} on {p.device}")
         if not (g.is_contiguous() and p.is_contiguous()) and not (_dense(g) and _same_order(g, p)):
@@ -412,7 +412,7 @@ def _clip_call(grads, max_norm: float, grad_scale) -> torch.Tensor:
             _written(grads)
         return norm
     for i, g in enumerate(grads):
-        if g.is_sparse:
+        if g.layout != torch.strided:
             _refuse(f"grads[{i}] is sparse")
     kinds = _kinds(grads)
     flat = [g if _dense(g) else g.contiguous() for g in grads]
@@ -659,19 +659,26 @@ class AdamW:
         self._lists = tuple([None] * len(flat) for _ in range(4))
         for k, st in sd["state"].items():
             p = flat[int(k)]
-            if tuple(st["exp_avg"].shape) != tuple(p.shape):
-                raise ValueError(f"loaded moments of parameter {k} have shape {tuple(st['exp_avg'].shape)}, the parameter {tuple(p.shape)}")
-            if "root" in st:
-                new = {"exp_avg": like(st["exp_avg"].view(torch.uint8), p, torch.uint8).view(_F8), "exp_avg_scale": st["exp_avg_scale"].detach().to(p.device).clone(),
-                       "root": like(st["root"].view(torch.uint8), p, torch.uint8).view(_F8), "root_scale": st["root_scale"].detach().to(p.device).clone()}
+            have = 8 if "root" in st else 32
+            blocks, codes = -(-p.numel() // STATE8_BLOCK), ("exp_avg", "root") if have == 8 else ("exp_avg", "exp_avg_sq")
+            if any(tuple(st[c].shape) != tuple(p.shape) for c in codes) or \
+                    (have == 8 and any(st[c].dtype != _F8 or st[c + "_scale"].dtype != torch.float32 or tuple(st[c + "_scale"].shape) != (blocks,) for c in codes)):
+                raise ValueError(f"loaded moments of parameter {k} ({[(c, st[c].dtype, tuple(st[c].shape)) for c in codes]}) do not fit the parameter {tuple(p.shape)}")
+            if have == 8:                            # in their own memory order: a scale belongs to consecutive elements
+                at = lambda t: t.detach().to(p.device, copy=True)  # noqa: E731
+                st8 = AdamState8([at(st["exp_avg"].view(torch.uint8)).view(_F8)], [at(st["exp_avg_scale"]).contiguous()],
+                                 [at(st["root"].view(torch.uint8)).view(_F8)], [at(st["root_scale"]).contiguous()])
+                new = dict(zip(AdamState8._fields, (x[0] for x in st8)))
+                if self._bits(p) == 32 or not all(_dense(new[c]) and _same_order(new[c], p) for c in codes):
+                    full = [torch.empty_like(new["exp_avg"], dtype=torch.float32) for _ in range(2)]
+                    read_adam_state8(st8, full[:1], full[1:])
+                    new = {"exp_avg": like(full[0], p, torch.float32), "exp_avg_sq": like(full[1], p, torch.float32)}
             else:
-                new = {"exp_avg": like(st["exp_avg"], p, torch.float32), "exp_avg_sq": like(st["exp_avg_sq"], p, torch.float32)}
-            have = 8 if "root" in new else 32
-            if have != self._bits(p):
-                st8 = AdamState8.zeros([p]) if have == 32 else AdamState8(*([new[f]] for f in AdamState8._fields))
-                full = [new["exp_avg"], new["exp_avg_sq"]] if have == 32 else [torch.empty_like(p, dtype=torch.float32) for _ in range(2)]
-                (write_adam_state8 if have == 32 else read_adam_state8)(st8, full[:1], full[1:])
-                new = dict(zip(AdamState8._fields, (x[0] for x in st8))) if have == 32 else dict(zip(("exp_avg", "exp_avg_sq"), full))
+                new = {c: like(st[c], p, torch.float32) for c in codes}
+            if "root" not in new and self._bits(p) == 8:
+                st8 = AdamState8.zeros([p])
+                write_adam_state8(st8, [new["exp_avg"]], [new["exp_avg_sq"]])
+                new = dict(zip(AdamState8._fields, (x[0] for x in st8)))
             self._set_state(p, new)
             self._counts(p.device)[self._slot[p]] = int(st["step"])
         for g, src in zip(self.param_groups, groups):

@@ -626,6 +626,42 @@ def test_checkpoints_convert(have, want):
     t.step()
 
 
+def test_checkpoint_of_another_memory_order():
+    """8-bit moments belong to consecutive elements: a checkpoint whose parameters lay in channels-last order loads into contiguous ones by value."""
+    w = torch.randn(8, 16, 3, 3, 3, generator=gen(70), device=DEV)
+    g = torch.randn(8, 16, 3, 3, 3, generator=gen(71), device=DEV) * torch.exp2(torch.arange(16, device=DEV).float() - 8).view(1, 16, 1, 1, 1)
+    p, q = torch.nn.Parameter(w.contiguous(memory_format=torch.channels_last_3d)), torch.nn.Parameter(w.clone())
+    a, b = O.AdamW([p], state_bits=8, min_8bit_numel=1), O.AdamW([q], state_bits=8, min_8bit_numel=1)
+    p.grad = g.contiguous(memory_format=torch.channels_last_3d)
+    a.step()
+    b.load_state_dict(a.state_dict())
+    x, y = a.state_dict(bits=32)["state"][0], b.state_dict(bits=32)["state"][0]
+    assert b.state_dict()["state"][0]["exp_avg"].is_contiguous()
+    top = g.abs().max() * 0.1
+    # one more rounding to nearest: 2^-4 of a value, or 2^-10 of a block's scale (at most the tensor's) below the normal codes
+    assert bool(((x["exp_avg"] - y["exp_avg"]).abs() <= 1.001 * torch.maximum(2.0 ** -4 * x["exp_avg"].abs(), 2.0 ** -10 * top / 448)).all())
+    rx, ry = x["exp_avg_sq"].double().sqrt(), y["exp_avg_sq"].double().sqrt()
+    assert bool(((rx - ry).abs() <= 1.001 * torch.maximum(2.0 ** -4 * rx, 2.0 ** -9 * rx.max() / 448)).all())
+    q.grad = g.clone()
+    b.step()
+    assert bool(torch.isfinite(q).all())
+
+
+def test_checkpoints_that_do_not_fit():
+    p = torch.nn.Parameter(torch.randn(700, device=DEV))
+    p.grad = torch.randn_like(p)
+    for bits in (8, 32):
+        opt = O.AdamW([p], state_bits=bits, min_8bit_numel=1)
+        opt.step()
+        good = opt.state_dict()
+        for k, bad in (("exp_avg", torch.zeros(699, device=DEV)), ("root_scale", torch.zeros(2, device=DEV)), ("exp_avg_scale", torch.zeros(3, device=DEV, dtype=torch.float64)),
+                       ("root", torch.zeros(700, device=DEV)), ("exp_avg_sq", torch.zeros(1, device=DEV))):
+            st = good["state"][0]
+            if k in st:
+                with pytest.raises(ValueError, match="do not fit"):
+                    O.AdamW([p], state_bits=bits).load_state_dict({**good, "state": {0: {**st, k: bad}}})
+
+
 def test_optimizer_with_two_rates_clips_by_one_norm():
     net = network(3)
     ps = list(net.parameters())
