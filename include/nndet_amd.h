@@ -721,7 +721,7 @@ typedef struct NndetAdamw {
     const float* lr_device;     /* not NULL: the rate is read there instead (a captured step follows a schedule) */
     const float* grad_scale;    /* not NULL: the gradients carry this loss scale (torch.amp.GradScaler); they are divided by it */
     const float* found_inf;     /* not NULL and not 0 on the device: nothing but norm is written */
-    float* norm;                /* max_norm >= 0: [1] global 2-norm of the gradients without their scale, written (or NULL), or ... */
+    float* norm;                /* max_norm >= 0: [1] global 2-norm of the gradients without their scale, written (or NULL; none of the scalars above), or ... */
     int64_t norm_given;         /* ... not 0: read instead of computed (a norm over more tensors than this call's) */
     int32_t* steps;             /* step counts, advanced on the device */
 } NndetAdamw;

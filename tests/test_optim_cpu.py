@@ -150,6 +150,19 @@ def test_the_library_checks_its_arguments():
     assert lib.nndet_opt_workspace_bytes(-1) == 0 and lib.nndet_opt_workspace_bytes(2) > lib.nndet_opt_workspace_bytes(1) > 0
 
 
+def test_the_library_refuses_a_norm_that_is_one_of_its_inputs():
+    lib = L.load()
+    one = (L.NndetOptTensor * 1)()
+    one[0].param = one[0].grad = one[0].exp_avg = one[0].exp_avg_sq = 16
+    one[0].numel, one[0].state_bits = 4, 32
+    ws = (C.c_char * (1 << 18))()
+    for field in ("grad_scale", "lr_device", "found_inf"):
+        a = L.NndetAdamw(1e-3, 0.9, 0.999, 1e-8, 1.0)
+        a.steps, a.norm = 16, 32
+        setattr(a, field, 32)
+        assert lib.nndet_adamw_step(one, 1, C.byref(a), (C.addressof(ws) + 15) // 16 * 16, 1 << 17, None) == -1, field
+
+
 def test_optimizer_refuses():
     p = [torch.nn.Parameter(torch.zeros(5)), torch.nn.Parameter(torch.zeros(3))]
     for kw, match in ((dict(state_bits=16), "state_bits"), (dict(max_norm=-1.0), "max_norm"), (dict(weight_decay=-0.1), "weight_decay"), (dict(betas=(0.9, 1.0)), "betas"),

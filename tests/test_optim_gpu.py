@@ -422,6 +422,54 @@ def test_norm_and_clip(dtype, shift, sizes):
     assert all(guards_intact(v, b, shift) for v, b in x["buf"])
 
 
+BETWEEN = [4097, 8191, 8192, 300]                    # one launch for the step, several for the norm
+TILE = 4096                                          # of clipping alone (the step's: 2048)
+
+
+@pytest.mark.parametrize("sizes", [BETWEEN, BETWEEN + [8193]])
+def test_sizes_around_the_kernels_for_small_tensors(sizes):
+    for dtype in (torch.float32, torch.bfloat16):
+        for shift in (0, 1):
+            test_adamw_step(dtype, shift, 3, sizes)
+            test_adamw8_step(dtype, shift, 3, sizes)
+            test_norm_and_clip(dtype, shift, sizes)
+    test_state8_write_and_read(1, sizes)
+
+
+@pytest.mark.parametrize("sizes", [[TILE * 1023], [TILE * 1023 + 1], [70000] + [5] * 163, [70000] + [5] * 164, [0, 70000, 0, 0, 3] * 32 + [0, 4097]])
+def test_norm_and_clip_of_many_tiles_and_tensors(sizes):
+    """Few and many partial sums; one type in the kernel arguments and more tensors than they hold, empty ones in between and at the end.
+    (test_norm_and_clip adds two tensors, of 0 and 1 elements: 1024 and 1025 tiles, 166 and 167 tensors.)"""
+    for dtype in (torch.float32, torch.float16):
+        test_norm_and_clip(dtype, 1, sizes)
+
+
+@pytest.mark.parametrize("tiles", [1000, 1030])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_one_norm_over_tensors_of_three_types(tiles, bits):
+    """The partial sums of every type, in few workgroups (1000 tiles) and in many: all kernels behind them take the same factor."""
+    parts = [make([2048 * k, 77, 1, 5000], dtype, seed=40 + k) for k, dtype in ((tiles - 60, torch.float32), (20, torch.bfloat16), (25, torch.float16))]
+    x = {k: [t for part in parts for t in part[k]] for k in "pgmv"}
+    kinds = [t.dtype for t in x["p"]]
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in x["g"]))
+    factor = 0.25 * norm / (norm + 1e-6)
+    steps = torch.full((len(kinds),), 4, dtype=torch.int32, device=DEV)
+    if bits == 8:
+        st = O.AdamState8.zeros(x["p"])
+        want = [formula(p, g, m * 0, v * 0, 5, 1e-2, 0.9, 0.999, 1e-8, 0.1, factor) for p, g, m, v in zip(x["p"], x["g"], x["m"], x["v"])]
+        got = O.adamw8_step(x["p"], x["g"], st, steps, lr=1e-2, weight_decay=0.1, max_norm=0.25 * norm)
+    else:
+        want = [formula(p, g, m, v, 5, 1e-2, 0.9, 0.999, 1e-8, 0.1, factor) for p, g, m, v in zip(x["p"], x["g"], x["m"], x["v"])]
+        got = O.adamw_step(x["p"], x["g"], x["m"], x["v"], steps, lr=1e-2, weight_decay=0.1, max_norm=0.25 * norm)
+    assert abs(float(got) - norm) <= 2 * U * norm
+    for p, dtype, (wp, _, _) in zip(x["p"], kinds, want):
+        within(p, wp[0], 1.5 * wp[1], dtype)
+    clipped = [g.double() * factor for g in x["g"]]
+    assert abs(float(O.clip_grads_(x["g"], 0.25 * norm)) - norm) <= 2 * U * norm
+    for g, w, dtype in zip(x["g"], clipped, kinds):
+        within(g, w, 4 * U * w.abs() + 2.0 ** -149, dtype)
+
+
 def test_norm_of_extremes():
     n = lambda *v: float(O.grad_norm([torch.tensor(v, device=DEV)]))  # noqa: E731
     assert n(0.0) == 0.0 and n(3e38, 1e30) == pytest.approx(3e38) and n(1e-30, 0.0) == pytest.approx(1e-30, rel=1e-6)
