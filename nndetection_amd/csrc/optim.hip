@@ -5,7 +5,8 @@
 // a tensor, up to 99 of them a launch (166 gradients), so that every later kernel is ONE launch whatever n is), advances the step counts and works out what
 // is the same for a whole tensor. Then one launch per storage kind (type of the parameters x bits of the moments) has a workgroup for each
 // tile of 2048 consecutive elements of a tensor; no tile spans two tensors. A wave owns blocks of 256 consecutive elements, which are also
-// the blocks that share a scale of the 8-bit moments: the maximum never leaves the wave. Calls of few small tensors skip the table.
+// the blocks that share a scale of the 8-bit moments: the maximum never leaves the wave. Calls of few small tensors skip the table,
+// and clipping of tensors of one type does; a clipped step writes it in the norm's launch if its tensors are of one kind and fit the arguments.
 //
 // AdamW, t = count + 1, g' = g * factor (factor = clip / loss scale):
 //   m = b1 m + (1 - b1) g'        v = b2 v + (1 - b2) g'^2
@@ -40,15 +41,18 @@ static constexpr int OPT_GRID = 1 << 20;
 static constexpr int OPT_PARTIALS = 2048;        // workgroups (and fp64 partial sums) of the norm per storage kind (1024: 1 - 2 % slower)
 // A norm of up to OPT_INLINE_TILES tiles is cut into at most OPT_INLINE partial sums, which every workgroup behind it adds up by itself: one launch
 // less, 3 us of host time and 1 - 3 us of GPU time (an AdamW step of 10 tensors of 8000 elements with clipping 20.7 / 10.6 -> 17.8 / 9.3 us of host / GPU
-// time). With more tiles so few workgroups take longer than the launch, and more partial sums are too many to add up everywhere.
+// time, and 15.4 / 7.6 with the table written by k_opt_sumsq_own). With more tiles so few workgroups take longer than the launch, and more partial sums are too many to add up everywhere.
 static constexpr int OPT_INLINE = 256, OPT_INLINE_TILES = 1024;
 static constexpr int OPT_NORM_WG = 1024;         // threads of the workgroup that adds them up
 // The kernels for few small tensors (16 waves a tensor) take one type, as many tensors as the kernel arguments hold, none above OPT_FEW elements: at 8000
 // elements a tensor 11.1 / 5.7 us of host / GPU time with them and 13.5 / 6.3 without (10 tensors), at 16000 10.8 / 8.0 and 13.7 / 6.1: a replayed graph
-// would lose. A norm in ONE workgroup (OPT_FEW_NORM elements a tensor, OPT_FEW_TOTAL in all): 60 tensors of 1000 elements 6.5 us, 5.6 over many
-// workgroups and 3 us more of host time for the second launch.
-static constexpr int OPT_FEW = 8192, OPT_FEW_WG = 1024, OPT_FEW_NORM = 4096;
-static constexpr int64_t OPT_FEW_TOTAL = 65536;
+// would lose.
+static constexpr int OPT_FEW = 8192, OPT_FEW_WG = 1024;
+// A norm in ONE workgroup, elements a tensor and in all. Clipping alone saves the second launch, 3 us of host time (60 tensors of 1000 elements 12.6 / 6.7 us
+// of host / GPU time, 15.6 / 5.7 over many workgroups). A clipped step has two launches either way: 10 tensors of 1000 elements 6.8 us of GPU time, 7.6
+// over many workgroups, 60 of them 10.2 and 8.3.
+struct OptFewNorm { int most; int64_t total; };
+static constexpr OptFewNorm OPT_FEW_CLIP = {4096, 65536}, OPT_FEW_STEP = {2048, 16384};
 
 struct OptEntry {                                // one tensor in the workspace's table
     void* p; const void* g; void* m; void* v; float* ms; float* rs;
@@ -97,9 +101,7 @@ template <int PTRS> __device__ __forceinline__ OptCoef opt_coef(const OptTableAr
 template <int PTRS> __device__ __forceinline__ bool opt_skip(const OptTableArgs<PTRS>& A) { return A.found_inf && *A.found_inf != 0.0f; }
 template <int PTRS> __device__ __forceinline__ float opt_factor(const OptTableArgs<PTRS>& A) { return A.grad_scale ? (float)(1.0 / (double)*A.grad_scale) : 1.0f; }
 
-template <int PTRS>
-__global__ __launch_bounds__(192) void k_opt_table(const OptTableArgs<PTRS> A) {
-    const int i = threadIdx.x;
+template <int PTRS> __device__ __forceinline__ void opt_write_table(const OptTableArgs<PTRS>& A, int i) {
     const bool skip = opt_skip(A);
     if (A.first && i == 0) {
         A.head->skip = skip;
@@ -123,6 +125,8 @@ __global__ __launch_bounds__(192) void k_opt_table(const OptTableArgs<PTRS> A) {
     A.coef[i] = opt_coef(A, a.wd, t);
     opt_stored();
 }
+template <int PTRS>
+__global__ __launch_bounds__(192) void k_opt_table(const OptTableArgs<PTRS> A) { opt_write_table(A, threadIdx.x); }
 
 // The table is written by an earlier kernel and constant in this one: read it through the scalar cache, so that what is uniform for a
 // workgroup stays in scalar registers (the compiler cannot see that the kernel's own stores do not touch it).
@@ -179,11 +183,11 @@ __device__ __forceinline__ bool opt_vectors(const OptEntry& e, int size, bool pa
 // chip works on neighbouring addresses. The tensor is looked up again only when the walk leaves it.
 template <int NB, typename S> struct OptWalk {
     static constexpr int TILE = NB * 4 * OPT_BLOCK;
-    const S src; uint32_t tiles, tile, start, end;
+    const S src; uint32_t tiles, step, tile, start, end;
     int i;
     OptEntry cur;
-    __device__ OptWalk(const S& s, uint32_t tiles_) : src(s), tiles(tiles_), tile(blockIdx.x), end(0), i(-1) {}
-    __device__ __forceinline__ void next() { tile += gridDim.x; }
+    __device__ OptWalk(const S& s, uint32_t tiles_, uint32_t wgs = gridDim.x) : src(s), tiles(tiles_), step(wgs), tile(blockIdx.x), end(0), i(-1) {}
+    __device__ __forceinline__ void next() { tile += step; }
     __device__ __forceinline__ bool enter() {    // true if the tile is another tensor's than the last one
         if (tile < end) return false;
         i = opt_find(src, tile);
@@ -464,11 +468,11 @@ template <bool FULL, int U, typename T> __device__ __forceinline__ double opt_su
         for (int k = 0; k < 4; ++k) s = fma((double)g[u][k], (double)g[u][k], s);
     return s;
 }
-template <typename T, int NB, typename S> __device__ __forceinline__ void opt_sumsq_walk(const S& src, uint32_t tiles, double* partial) {
+template <typename T, int NB, typename S> __device__ __forceinline__ void opt_sumsq_walk(const S& src, uint32_t tiles, uint32_t wgs, double* partial) {
     __shared__ double part[OPT_WG / 64];
     const int lane = threadIdx.x & 63;
     double s = 0.0;
-    OptWalk<NB, S> w(src, tiles);
+    OptWalk<NB, S> w(src, tiles, wgs);
     opt_blocks<NB, NB>(w, [&] { return opt_vectors(w.cur, sizeof(T), false, 0); },
                        [&](auto kind, int64_t base, int rem) { s = opt_sumsq<kind.FULL, kind.N, T>(w.cur, base, rem, lane, s); });
     s = wave_sum_f64(s);
@@ -477,10 +481,13 @@ template <typename T, int NB, typename S> __device__ __forceinline__ void opt_su
     if (threadIdx.x == 0) partial[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 template <typename T, int NB>
-__global__ __launch_bounds__(OPT_WG) void k_opt_sumsq(OptMem src, uint32_t tiles, double* partial) { opt_sumsq_walk<T, NB>(src, tiles, partial); }
-template <typename T>
-__global__ __launch_bounds__(OPT_WG) void k_opt_sumsq_own(const OptTableArgs<1> A, uint32_t tiles, double* partial) {
-    opt_sumsq_walk<T, OPT_CLIP_NB>(OptOwn<1>{A, A.n}, tiles, partial);
+__global__ __launch_bounds__(OPT_WG) void k_opt_sumsq(OptMem src, uint32_t tiles, double* partial) { opt_sumsq_walk<T, NB>(src, tiles, gridDim.x, partial); }
+// The same with the tensors in the kernel arguments. A step (PTRS > 1) needs the table in the kernel behind: a workgroup of its own, the last, writes it.
+template <typename T, int NB, int PTRS>
+__global__ __launch_bounds__(OPT_WG) void k_opt_sumsq_own(const OptTableArgs<PTRS> A, uint32_t tiles, double* partial) {
+    const uint32_t wgs = gridDim.x - (PTRS > 1);
+    if (PTRS > 1 && blockIdx.x == wgs) opt_write_table(A, threadIdx.x);
+    else opt_sumsq_walk<T, NB>(OptOwn<PTRS>{A, A.n}, tiles, wgs, partial);
 }
 
 // The norm (count < 0: given at norm_at) and the factor. One workgroup, a launch of its own: 4 us. Finishing in the last workgroup of k_opt_sumsq
@@ -564,7 +571,7 @@ __global__ __launch_bounds__(OPT_WG) void k_opt_state8(OptMem src, uint32_t tile
 }
 
 // ---- few small tensors: no table. The tensors are read from the kernel arguments by the kernel that works on them, one workgroup a tensor, which
-// also advances its count: one launch instead of two (with clipping two instead of four; clipping alone one instead of four). A launch costs 4 us of
+// also advances its count: one launch instead of two (clipping alone one instead of two; a clipped step two either way). A launch costs 4 us of
 // host time and 2 - 4 us of GPU time, which is what such a call consists of.
 template <typename T, int BITS>
 __global__ __launch_bounds__(OPT_FEW_WG) void k_adamw_few(const OptTableArgs<BITS == 8 ? 6 : 4> A, OptHyper H, int clipped) {
@@ -760,23 +767,30 @@ static inline unsigned opt_grid(int64_t tiles, int most) { return (unsigned)(til
 
 static OptMem opt_mem(const OptPlan& P, int k) { return {P.entry + P.first[k], P.tile0 + P.first[k], P.first[k + 1] - P.first[k]}; }
 
-// The norm's launches. N: what the kernels behind them need (N.count 0: the factor is in the head).
-template <int NB> static int opt_norm(const OptPlan& P, const float* grad_scale, double max_norm, float* norm, bool given, OptSums& N, hipStream_t st) {
+// The norm's launches. own: all tensors, of one type, with PTRS addresses each (0: none; above 1 the table is written on the way). N: what the kernels behind them need
+// (N.count 0: the factor is in the head).
+template <int NB, int PTRS>
+static int opt_norm(const OptPlan& P, const OptTableArgs<PTRS ? PTRS : 1>* own, const float* grad_scale, double max_norm, float* norm, bool given, OptSums& N, hipStream_t st) {
     int64_t tiles = 0;
     int kinds = 0, count = 0;
     for (int k = 0; k < 6; ++k) tiles += P.tiles[k], kinds += P.tiles[k] != 0;
     N = {P.partial, 0, grad_scale, max_norm, norm};
-    const bool own = !given && kinds && max_norm >= 0.0 && tiles <= OPT_INLINE_TILES;
+    const bool finish = given || !kinds || max_norm < 0.0 || tiles > OPT_INLINE_TILES;
     for (int k = 0; k < 6 && !given; ++k) {
         if (!P.tiles[k]) continue;
-        const unsigned g = opt_grid(P.tiles[k], own ? OPT_INLINE / kinds : OPT_PARTIALS);
+        const unsigned g = opt_grid(P.tiles[k], finish ? OPT_PARTIALS : OPT_INLINE / kinds);
+#define OPT_OWN(T) (k_opt_sumsq_own<T, NB, PTRS><<<g + (PTRS > 1), OPT_WG, 0, st>>>(*own, (uint32_t)P.tiles[k], P.partial))
 #define OPT_CALL(T) (k_opt_sumsq<T, NB><<<g, OPT_WG, 0, st>>>(opt_mem(P, k), (uint32_t)P.tiles[k], P.partial + count))
-        NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL);
+        if constexpr (PTRS != 0)
+            if (own) NNDET_DISPATCH_DTYPE(k % 3, OPT_OWN);
+        if constexpr (PTRS < 2)
+            if (!own) NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL);
+#undef OPT_OWN
 #undef OPT_CALL
         LAUNCH_CHECK();
         count += (int)g;
     }
-    if (own) {
+    if (!finish) {
         N.count = count;
         return 0;
     }
@@ -785,13 +799,39 @@ template <int NB> static int opt_norm(const OptPlan& P, const float* grad_scale,
     return 0;
 }
 
+// The plan of a call whose tensors are of one kind and in A; false if they are not (or are all empty).
+template <int PTRS>
+static bool opt_own(const NndetOptTensor* t, int32_t n, const OptScalars& S, int nb, OptPlan& P, OptTableArgs<PTRS>& A) {
+    const int kind = opt_few(t, n, INT64_MAX, INT64_MAX, S, P, A);
+    if (kind < 0) return false;
+    int64_t tiles = 0;
+    for (int i = 0; i < n; ++i) {
+        A.a[i].tile0 = (uint32_t)tiles;
+        tiles += ceil_div64(t[i].numel, nb * 4 * OPT_BLOCK);
+    }
+    for (int k = 0; k < 7; ++k) P.first[k] = k <= kind ? 0 : n;
+    for (int k = 0; k < 6; ++k) P.tiles[k] = k == kind ? tiles : 0;
+    return tiles != 0;
+}
+
+// The norm of a step, with the table: one launch if the tensors fit the kernel arguments.
+template <int PTRS>
+static int adamw_norm(const NndetOptTensor* t, int32_t n, const NndetAdamw* a, const OptScalars& S, OptPlan& P, OptSums& N, hipStream_t st, bool* done) {
+    OptTableArgs<PTRS> A;
+    *done = opt_own(t, n, S, OPT_NB, P, A);
+    if (!*done) return 0;
+    A.entry = P.entry; A.coef = P.coef; A.tile0 = P.tile0;
+    A.first = 1;
+    return opt_norm<OPT_NB, PTRS>(P, &A, a->grad_scale, a->max_norm, a->norm, false, N, st);
+}
+
 // An AdamW step of few tensors: true if it was one (its return code in rc).
 template <int BITS>
 static bool adamw_few(const NndetOptTensor* t, int32_t n, const NndetAdamw* a, const OptScalars& S, const OptHyper& H, OptPlan& P, hipStream_t st, int* rc) {
     OptTableArgs<BITS == 8 ? 6 : 4> A;
     const bool clip = a->max_norm >= 0.0;
     if (clip && a->norm_given) return false;
-    const int k = opt_few(t, n, clip ? OPT_FEW_NORM : OPT_FEW, clip ? OPT_FEW_TOTAL : INT64_MAX, S, P, A);
+    const int k = opt_few(t, n, clip ? OPT_FEW_STEP.most : OPT_FEW, clip ? OPT_FEW_STEP.total : INT64_MAX, S, P, A);
     if (k < 0) return false;
 #define OPT_NORM(T) (k_opt_norm_few<T, false><<<1, OPT_FEW_WG, 0, st>>>(A, a->max_norm, a->norm))
 #define OPT_CALL(T) (k_adamw_few<T, BITS><<<n, OPT_FEW_WG, 0, st>>>(A, H, clip))
@@ -814,11 +854,16 @@ extern "C" int nndet_adamw_step(const NndetOptTensor* tensors, int32_t n, const 
     OptPlan P;
     int rc = opt_check(tensors, n, 7, workspace, workspace_bytes, P);
     if (rc || adamw_few<32>(tensors, n, a, S, H, P, st, &rc) || adamw_few<8>(tensors, n, a, S, H, P, st, &rc)) return rc;
-    rc = opt_begin(tensors, n, S, OPT_NB, P, st);
-    if (rc) return rc;
     OptSums N = {};
-    if (a->max_norm >= 0.0) {
-        rc = opt_norm<OPT_NB>(P, a->grad_scale, a->max_norm, a->norm, a->norm_given != 0, N, st);
+    bool own = false;
+    if (a->max_norm >= 0.0 && !a->norm_given) {
+        rc = adamw_norm<4>(tensors, n, a, S, P, N, st, &own);
+        if (!rc && !own) rc = adamw_norm<6>(tensors, n, a, S, P, N, st, &own);
+        if (rc) return rc;
+    }
+    if (!own) {
+        rc = opt_begin(tensors, n, S, OPT_NB, P, st);
+        if (!rc && a->max_norm >= 0.0) rc = opt_norm<OPT_NB, 0>(P, nullptr, a->grad_scale, a->max_norm, a->norm, a->norm_given != 0, N, st);
         if (rc) return rc;
     }
     for (int k = 0; k < 6; ++k) {
@@ -836,34 +881,6 @@ extern "C" int nndet_adamw_step(const NndetOptTensor* tensors, int32_t n, const 
     return 0;
 }
 
-// Clipping of tensors of one type that fit the kernel arguments: no table (10 tensors of 8000 elements 18.5 / 8.8 -> 13.5 / 5.3 us of host / GPU time with
-// the norm's finish in the scaling kernel; the two kernels themselves take the same time as with a table).
-static int opt_clip_own(int kind, const NndetOptTensor* t, int32_t n, double max_norm, const float* grad_scale, float* norm_out, OptPlan& P, OptTableArgs<1>& A, hipStream_t st) {
-    int64_t tiles = 0;
-    for (int i = 0; i < n; ++i) {
-        A.a[i].tile0 = (uint32_t)tiles;
-        tiles += ceil_div64(t[i].numel, OPT_CLIP_NB * 4 * OPT_BLOCK);
-    }
-    OptSums N = {P.partial, 0, grad_scale, max_norm, norm_out};
-    const bool own = max_norm >= 0.0 && tiles <= OPT_INLINE_TILES;
-    const unsigned g = opt_grid(tiles, own ? OPT_INLINE : OPT_PARTIALS);
-#define OPT_SUM(T) (k_opt_sumsq_own<T><<<g, OPT_WG, 0, st>>>(A, (uint32_t)tiles, P.partial))
-#define OPT_CALL(T) (k_opt_scale_own<T><<<opt_grid(tiles, OPT_GRID), OPT_WG, 0, st>>>(A, (uint32_t)tiles, N))
-    NNDET_DISPATCH_DTYPE(kind % 3, OPT_SUM);
-    LAUNCH_CHECK();
-    if (own) N.count = (int)g;
-    else {
-        k_opt_norm<<<1, OPT_NORM_WG, 0, st>>>(P.partial, (int)g, grad_scale, max_norm, norm_out, P.head);
-        LAUNCH_CHECK();
-    }
-    if (max_norm < 0.0) return 0;                // the norm alone
-    NNDET_DISPATCH_DTYPE(kind % 3, OPT_CALL);
-#undef OPT_SUM
-#undef OPT_CALL
-    LAUNCH_CHECK();
-    return 0;
-}
-
 extern "C" int nndet_grad_clip(const NndetOptTensor* tensors, int32_t n, double max_norm, const float* grad_scale, float* norm_out, void* workspace, size_t workspace_bytes, void* stream) {
     if (max_norm != max_norm || !norm_out || (grad_scale && max_norm >= 0.0)) return NNDET_EINVAL;
     hipStream_t st = as_stream(stream);
@@ -874,7 +891,7 @@ extern "C" int nndet_grad_clip(const NndetOptTensor* tensors, int32_t n, double 
     for (int i = 0; i < n; ++i)
         if (tensors[i].state_bits != 32) return NNDET_EINVAL;
     OptTableArgs<1> A;
-    const int few = opt_few(tensors, n, OPT_FEW_NORM, OPT_FEW_TOTAL, {nullptr, nullptr, nullptr, grad_scale, 0.0, 0.0, 0.0}, P, A);
+    const int few = opt_few(tensors, n, OPT_FEW_CLIP.most, OPT_FEW_CLIP.total, {nullptr, nullptr, nullptr, grad_scale, 0.0, 0.0, 0.0}, P, A);
     if (few >= 0) {
 #define OPT_CALL(T) (k_opt_norm_few<T, true><<<1, OPT_FEW_WG, 0, st>>>(A, max_norm, norm_out))
         NNDET_DISPATCH_DTYPE(few % 3, OPT_CALL);
@@ -882,18 +899,21 @@ extern "C" int nndet_grad_clip(const NndetOptTensor* tensors, int32_t n, double 
         LAUNCH_CHECK();
         return 0;
     }
-    const int own = opt_few(tensors, n, INT64_MAX, INT64_MAX, S, P, A);
-    if (own >= 0) return opt_clip_own(own, tensors, n, max_norm, grad_scale, norm_out, P, A, st);
-    rc = opt_begin(tensors, n, S, OPT_CLIP_NB, P, st, true);
-    if (rc) return rc;
+    // Tensors of one type that fit the kernel arguments need no table (10 tensors of 8000 elements 18.5 / 8.8 -> 13.5 / 5.3 us of host / GPU time together
+    // with the norm's finish in the scaling kernel).
+    const bool own = opt_own(tensors, n, S, OPT_CLIP_NB, P, A);
+    if (!own && (rc = opt_begin(tensors, n, S, OPT_CLIP_NB, P, st, true))) return rc;
     OptSums N;
-    rc = opt_norm<OPT_CLIP_NB>(P, grad_scale, max_norm, norm_out, false, N, st);
+    rc = opt_norm<OPT_CLIP_NB, 1>(P, own ? &A : nullptr, grad_scale, max_norm, norm_out, false, N, st);
     if (rc || max_norm < 0.0) return rc;         // the norm alone
     for (int k = 0; k < 3; ++k) {
         if (!P.tiles[k]) continue;
         const unsigned g = opt_grid(P.tiles[k], OPT_GRID);
+#define OPT_OWN(T) (k_opt_scale_own<T><<<g, OPT_WG, 0, st>>>(A, (uint32_t)P.tiles[k], N))
 #define OPT_CALL(T) (k_opt_scale<T><<<g, OPT_WG, 0, st>>>(opt_mem(P, k), (uint32_t)P.tiles[k], P.head, N))
-        NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL);
+        if (own) NNDET_DISPATCH_DTYPE(k % 3, OPT_OWN);
+        else NNDET_DISPATCH_DTYPE(k % 3, OPT_CALL);
+#undef OPT_OWN
 #undef OPT_CALL
         LAUNCH_CHECK();
     }
