@@ -176,7 +176,7 @@ def _to8(x, root, pair=None, step=None):
     training step (`pair` given) rounds it up with the probability of its distance from the code below, by 16 bits an element that follow
     from its place and the step: a moving average that changes by 0.1 % a step would stand still under rounding to nearest."""
     scale = x.abs().amax(1, keepdim=True) * (1.0 / 448.0)
-    scale = torch.where(scale < 2.0 ** -110, 0.0, scale)
+    scale = torch.where(scale >= 2.0 ** -110, scale, 0.0)
     y = torch.where(scale > 0, x * (1.0 / scale), 0.0)
     if not root:
         return y.to(torch.float8_e4m3fn), scale
