@@ -281,10 +281,26 @@ __device__ __forceinline__ void opt_decode(uint32_t c, float s, float* x) {
 // One residual step behind the hardware's reciprocal (root): correctly rounded but for about one value in 2^22.
 __device__ __forceinline__ float opt_root(float v) {
     const float y = __builtin_amdgcn_rsqf(v), s = v * y;
-    const float r = fmaf(fmaf(-s, s, v), 0.5f * y, s);
-    return __builtin_amdgcn_classf(v, 0x100) ? r : v * 0x1p-24f;         // not a positive normal number: 0, inf and NaN are their own roots, denormals go to 0
+    return fmaf(fmaf(-s, s, v), 0.5f * y, s);
 }
-__device__ __forceinline__ float opt_quotient(float m, float d) {       // d is not a denormal: roots are 0 or above 2^-63, eps is 0 or normal, scales 0 or above 2^-110
+// Roots of four numbers >= 0. Below 2^-96 the residual falls out of the normal range, and below 2^-126 so does v itself: those are scaled by
+// 2^64 first, behind a branch that ordinary second moments never take (one test for the four: v - 1 as an integer sends 0 to the top).
+__device__ __forceinline__ void opt_roots(const float* v, float* r) {
+    constexpr uint32_t SMALL = (127 - 96) << 23;
+    uint32_t least = 0xffffffffu;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float x = opt_root(v[k]);
+        r[k] = __builtin_amdgcn_classf(v[k], 0x100) ? x : v[k];          // 0, inf and NaN are their own roots
+        least = min(least, __float_as_uint(v[k]) - 1);
+    }
+    if (least < SMALL - 1) {
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k)
+            if (__float_as_uint(v[k]) - 1 < SMALL - 1) r[k] = opt_root(v[k] * 0x1p64f) * 0x1p-32f;
+    }
+}
+__device__ __forceinline__ float opt_quotient(float m, float d) {       // d is not a denormal: roots are 0 or above 2^-75, eps is 0 or normal, scales 0 or above 2^-110
     const float y = __builtin_amdgcn_rcpf(d), q = m * y;
     return __builtin_amdgcn_div_fixupf(fmaf(fmaf(-d, q, m), y, q), d, m);
 }
@@ -417,7 +433,11 @@ __device__ __forceinline__ void adamw_block(const OptEntry& e, int64_t base, int
             g[u][k] = g[u][k] * factor;
             m[u][k] = m[u][k] * H.b1 + g[u][k] * H.omb1;
             v[u][k] = v[u][k] * H.b2 + (g[u][k] * g[u][k]) * H.omb2;
-            r[k] = BITS == 8 ? opt_root(v[u][k]) : sqrtf(v[u][k]);
+            if constexpr (BITS != 8) r[k] = sqrtf(v[u][k]);
+        }
+        if constexpr (BITS == 8) opt_roots(v[u], r);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
             const float den = r[k] * c.unbias + H.eps;
             p[u][k] = p[u][k] * c.decay - (BITS == 8 ? opt_quotient(m[u][k], den) : m[u][k] / den) * c.size;
         }

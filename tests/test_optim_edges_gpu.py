@@ -1,0 +1,54 @@
+"""GPU: calls of the optimiser's operators at the edges of what they accept: second moments below the normal range, tensor counts around the
+limits of every launch, steps that are replayed, state that is copied."""
+import math
+
+import pytest
+import torch
+
+from nndetection_amd import optim as O
+from tests.test_optim_gpu import BLOCK, DEV, U, check8, formula, gen, rows, within
+
+pytestmark = pytest.mark.gpu
+TINY = 2.0 ** -149                                   # one denormal step
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -126, 1e-24, 1e-8])
+@pytest.mark.parametrize("sizes", [[300, 1, 257], [70001, 5000, 300]])
+def test_second_moments_below_the_normal_range(bits, eps, sizes):
+    """Gradients of 2e-20 .. 3e-18: their squares times (1 - b2) are denormal (4e-43 .. 9e-39), the first step is about lr all the same, and so is
+    the second from the moments that the first has stored.
+
+    Beside `formula`'s roundings, which are relative, a denormal v is off by half a step of 2^-149 for each operation that makes it (square, two
+    products, sum, and with 8 bits the square of the stored root): ev <= 6.06 u v (9.09 with 8 bits) + 2.5 steps. Here v >= 285 steps at the first step, so ev / v
+    <= 0.9 %; at the second v is at least 0.999 of that (32 bits), or of the squared least stored root (a code is at most 1/2 below its value
+    where codes are denormal: v >= 70 steps, ev / v <= 3.6 %). The root is off by at most ev / v of itself (half, and second order), and
+    so is the quotient by at most ev / v / (1 - ev / v)."""
+    g = gen(5)
+    p = [torch.randn(n, generator=g, device=DEV) for n in sizes]
+    gr = [torch.exp2(torch.empty(n, device=DEV).uniform_(-65.4, -58.2, generator=g)) * torch.where(torch.rand(n, generator=g, device=DEV) < 0.5, -1.0, 1.0) for n in sizes]
+    steps = torch.zeros(len(sizes), dtype=torch.int32, device=DEV)
+    st = O.AdamState8.zeros(p)
+    m, v = [torch.zeros_like(x) for x in p], [torch.zeros_like(x) for x in p]
+    for t in (1, 2):
+        if bits == 8:
+            m = [(rows(c.float()).double() * s.double().view(-1, 1)).view(-1)[:c.numel()] for c, s in zip(st.exp_avg, st.exp_avg_scale)]
+            v = [(rows(c.float()).double() * s.double().view(-1, 1)).square().view(-1)[:c.numel()] for c, s in zip(st.root, st.root_scale)]
+        want = [formula(*x, t, 1e-3, 0.9, 0.999, eps, 0.1) for x in zip(p, gr, m, v)]
+        if bits == 8:
+            O.adamw8_step(p, gr, st, steps, lr=1e-3, eps=eps, weight_decay=0.1)
+        else:
+            O.adamw_step(p, gr, m, v, steps, lr=1e-3, eps=eps, weight_decay=0.1)
+        for i, (wp, wm, wv) in enumerate(want):
+            ev = 1.5 * wv[1] + 2.5 * TINY
+            off = ev / wv[0]
+            assert float(off.max()) < 0.04
+            size, unbias = 1e-3 / (1 - 0.9 ** t), 1 / math.sqrt(1 - 0.999 ** t)
+            q = wm[0].abs() / (wv[0].sqrt() * unbias + eps)
+            within(p[i], wp[0], 1.5 * wp[1] + size * q * off / (1 - off), what=f"p {sizes[i]} step {t}")
+            if bits == 8:
+                r = wv[0].sqrt()
+                check8(st, i, wm[0], 1.5 * wm[1], r, 6 * U * r + r * off, False)
+            else:
+                within(m[i], *wm)
+                within(v[i], wv[0], ev)
