@@ -536,7 +536,6 @@ class AdamW:
         self._slot = {p: i for i, p in enumerate(flat)}
         self._state = {}                             # parameter -> {name: tensor}
         self._steps = {}                             # device -> int32 counts, one for every parameter
-        self._fixed = {}                             # parameter -> addresses of its state, number of elements, last word of its struct
         self._flat = flat                            # in the order of the slots, and the state's tensors in that order (None: no state yet)
         self._lists = tuple([None] * len(flat) for _ in range(4))
 
@@ -561,12 +560,9 @@ class AdamW:
             self._set_state(p, {"exp_avg": torch.zeros_like(p, dtype=torch.float32), "exp_avg_sq": torch.zeros_like(p, dtype=torch.float32)})
 
     def _set_state(self, p, st: dict) -> None:
-        bits = 8 if "root" in st else 32
-        at = [st[k].data_ptr() if k in st else 0 for k in (("exp_avg", "root", "exp_avg_scale", "root_scale") if bits == 8 else ("exp_avg", "exp_avg_sq", "", ""))]
         self._state[p] = st
-        for ts, k in zip(self._lists, ("exp_avg", "root" if bits == 8 else "exp_avg_sq", "exp_avg_scale", "root_scale")):
+        for ts, k in zip(self._lists, ("exp_avg", "root" if "root" in st else "exp_avg_sq", "exp_avg_scale", "root_scale")):
             ts[self._slot[p]] = st.get(k)
-        self._fixed[p] = (*at, p.numel(), self._slot[p] | (bits << 48), p.stride(), p.device)
 
     @torch.no_grad()
     def step(self) -> None:
@@ -592,19 +588,20 @@ class AdamW:
                 gr = p.grad
                 if gr is None:
                     continue
-                fixed = self._fixed.get(p)
-                if fixed is None:
+                if p not in self._state:
                     self._init_state(p)
-                    fixed = self._fixed[p]
-                m, v, ms, rs, numel, tail, stride, device = fixed
-                if p.device != device or p.numel() != numel or p.stride() != stride:
+                slot = self._slot[p]
+                m, v, ms, rs = (ts[slot] for ts in self._lists)
+                device = m.device
+                if p.device != device or p.shape != m.shape or (p.stride() != m.stride() and not (_dense(p) and _same_order(p, m))):
                     _refuse(f"a parameter of shape {tuple(p.shape)} on {p.device} was moved or changed its size after its state was made")
-                tail |= _kinds([p])[0]               # (its type may have changed: the moments are fp32 or 8 bits whatever it is)
+                # (its type may have changed: the moments are fp32 or 8 bits whatever it is)
+                tail = slot | _kinds([p])[0] | ((32 if ms is None else 8) << 48)
                 gr = _grads_like([p], [gr])[0]
                 c = calls.get((device, key))
                 if c is None:
                     c = calls[(device, key)] = ([], [], [], g)
-                c[0].extend((p.data_ptr(), gr.data_ptr(), m, v, ms, rs, numel, wd, tail))
+                c[0].extend((p.data_ptr(), gr.data_ptr(), m.data_ptr(), v.data_ptr(), *((0, 0) if ms is None else (ms.data_ptr(), rs.data_ptr())), p.numel(), wd, tail))
                 c[1].append(p)
                 c[2].append(gr)
         if not calls:
@@ -655,7 +652,7 @@ class AdamW:
             raise ValueError("amsgrad and maximize are not supported")
         flat = [p for g in self.param_groups for p in g["params"]]
         like = lambda t, p, dtype: torch.empty_like(p, dtype=dtype).copy_(t.detach())  # noqa: E731
-        self._state, self._fixed, self._steps = {}, {}, {}
+        self._state, self._steps = {}, {}
         self._lists = tuple([None] * len(flat) for _ in range(4))
         for k, st in sd["state"].items():
             p = flat[int(k)]
