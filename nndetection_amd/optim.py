@@ -491,6 +491,12 @@ def read_adam_state8(state: AdamState8, exp_avgs, exp_avg_sqs) -> None:
     _state8_call(state, exp_avgs, exp_avg_sqs, 0)
 
 
+def _check_group(wd, betas, eps) -> None:
+    b1, b2 = betas
+    if not (wd >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and (eps == 0.0 or eps >= 2.0 ** -126)):
+        _refuse(f"weight_decay {wd} >= 0, betas {(b1, b2)} in [0, 1) and an eps {eps} that is 0 or a normal fp32 number are wanted")
+
+
 class AdamW:
     """AdamW on the operators above, with the interface of `SGDNesterov`: one call of the library a step for all parameters that share
     (lr, betas, eps), whatever their weight decays and types.
@@ -515,9 +521,7 @@ class AdamW:
         if groups and not isinstance(groups[0], dict):
             groups = [{"params": groups}]
         for g in [{"weight_decay": weight_decay, "betas": betas, "eps": eps}, *groups]:
-            wd, (b1, b2), e = g.get("weight_decay", 0.0), g.get("betas", betas), g.get("eps", eps)
-            if not (wd >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and (e == 0.0 or e >= 2.0 ** -126)):
-                _refuse(f"weight_decay {wd} >= 0, betas {(b1, b2)} in [0, 1) and an eps {e} that is 0 or a normal fp32 number are wanted")
+            _check_group(g.get("weight_decay", 0.0), g.get("betas", betas), g.get("eps", eps))
         self.defaults = {"lr": float(lr), "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay}
         self.param_groups = []
         for g in groups:
@@ -644,41 +648,66 @@ class AdamW:
                            "differentiable": False, "fused": None, "decoupled_weight_decay": True, "params": ids})
         return {"state": state, "param_groups": groups}
 
-    def load_state_dict(self, sd: dict) -> None:
+    def _check_loaded(self, sd: dict) -> None:
+        """Everything that load_state_dict wants of a checkpoint, before it touches the optimiser."""
         groups = sd["param_groups"]
         if len(groups) != len(self.param_groups) or any(len(a["params"]) != len(b["params"]) for a, b in zip(groups, self.param_groups)):
             raise ValueError("loaded state dict has different parameter groups")
         if any(g.get("amsgrad") or g.get("maximize") for g in groups):
             raise ValueError("amsgrad and maximize are not supported")
-        flat = [p for g in self.param_groups for p in g["params"]]
-        like = lambda t, p, dtype: torch.empty_like(p, dtype=dtype).copy_(t.detach())  # noqa: E731
-        self._state, self._steps = {}, {}
-        self._lists = tuple([None] * len(flat) for _ in range(4))
+        for i, g in enumerate(groups):
+            missing = [k for k in ("lr", "betas", "eps", "weight_decay") if k not in g]
+            if missing:
+                raise ValueError(f"loaded parameter group {i} has no {', '.join(missing)}")
+            float(g["lr"])
+            _check_group(float(g["weight_decay"]), g["betas"], float(g["eps"]))
         for k, st in sd["state"].items():
-            p = flat[int(k)]
-            have = 8 if "root" in st else 32
-            blocks, codes = -(-p.numel() // STATE8_BLOCK), ("exp_avg", "root") if have == 8 else ("exp_avg", "exp_avg_sq")
-            if any(tuple(st[c].shape) != tuple(p.shape) for c in codes) or \
-                    (have == 8 and any(st[c].dtype != _F8 or st[c + "_scale"].dtype != torch.float32 or tuple(st[c + "_scale"].shape) != (blocks,) for c in codes)):
-                raise ValueError(f"loaded moments of parameter {k} ({[(c, st[c].dtype, tuple(st[c].shape)) for c in codes]}) do not fit the parameter {tuple(p.shape)}")
-            if have == 8:                            # in their own memory order: a scale belongs to consecutive elements
+            if not 0 <= int(k) < len(self._flat):
+                raise ValueError(f"loaded state of parameter {k}: there are {len(self._flat)}")
+            p = self._flat[int(k)]
+            names = AdamState8._fields if "root" in st else ("exp_avg", "exp_avg_sq")
+            missing = [c for c in ("step", *names) if c not in st]
+            if missing:
+                raise ValueError(f"loaded state of parameter {k} has no {', '.join(missing)}")
+            if not 0 <= float(st["step"]) < 2 ** 31:
+                raise ValueError(f"loaded step {st['step']} of parameter {k}")
+            blocks = (-(-p.numel() // STATE8_BLOCK),)
+            for c in names:
+                scale = c.endswith("_scale")
+                if not isinstance(st[c], torch.Tensor) or tuple(st[c].shape) != (blocks if scale else tuple(p.shape)) or \
+                        ("root" in st and st[c].dtype != (torch.float32 if scale else _F8)):
+                    what = f"{st[c].dtype}, {tuple(st[c].shape)}" if isinstance(st[c], torch.Tensor) else type(st[c])
+                    raise ValueError(f"loaded moments of parameter {k} ({c}: {what}) do not fit the parameter {tuple(p.shape)}")
+
+    def load_state_dict(self, sd: dict) -> None:
+        """A checkpoint that does not fit is refused and changes nothing. The state is made anew: a captured step has to be captured again."""
+        self._check_loaded(sd)
+        like = lambda t, p, dtype: torch.empty_like(p, dtype=dtype).copy_(t.detach())  # noqa: E731
+        state, counts = {}, {}
+        for k, st in sd["state"].items():
+            p = self._flat[int(k)]
+            if "root" in st:                         # in their own memory order: a scale belongs to consecutive elements
                 at = lambda t: t.detach().to(p.device, copy=True)  # noqa: E731
                 st8 = AdamState8([at(st["exp_avg"].view(torch.uint8)).view(_F8)], [at(st["exp_avg_scale"]).contiguous()],
                                  [at(st["root"].view(torch.uint8)).view(_F8)], [at(st["root_scale"]).contiguous()])
                 new = dict(zip(AdamState8._fields, (x[0] for x in st8)))
-                if self._bits(p) == 32 or not all(_dense(new[c]) and _same_order(new[c], p) for c in codes):
+                if self._bits(p) == 32 or not all(_dense(new[c]) and _same_order(new[c], p) for c in ("exp_avg", "root")):
                     full = [torch.empty_like(new["exp_avg"], dtype=torch.float32) for _ in range(2)]
                     read_adam_state8(st8, full[:1], full[1:])
                     new = {"exp_avg": like(full[0], p, torch.float32), "exp_avg_sq": like(full[1], p, torch.float32)}
             else:
-                new = {c: like(st[c], p, torch.float32) for c in codes}
+                new = {c: like(st[c], p, torch.float32) for c in ("exp_avg", "exp_avg_sq")}
             if "root" not in new and self._bits(p) == 8:
                 st8 = AdamState8.zeros([p])
                 write_adam_state8(st8, [new["exp_avg"]], [new["exp_avg_sq"]])
                 new = dict(zip(AdamState8._fields, (x[0] for x in st8)))
+            state[p] = new
+            counts.setdefault(p.device, [0] * len(self._flat))[self._slot[p]] = int(st["step"])
+        steps = {device: torch.tensor(c, dtype=torch.int32, device=device) for device, c in counts.items()}
+        self._state, self._steps, self._lists = {}, steps, tuple([None] * len(self._flat) for _ in range(4))
+        for p, new in state.items():
             self._set_state(p, new)
-            self._counts(p.device)[self._slot[p]] = int(st["step"])
-        for g, src in zip(self.param_groups, groups):
+        for g, src in zip(self.param_groups, sd["param_groups"]):
             if isinstance(g["lr"], torch.Tensor):
                 g["lr"].fill_(float(src["lr"]))
             else:

@@ -49,3 +49,43 @@ def test_a_copied_optimizer_steps_its_own_state(monkeypatch, how):
             assert (t.param, t.grad, t.numel, t.slot, t.state_bits) == (p.data_ptr(), p.grad.data_ptr(), p.numel(), i, 32)
             assert (t.exp_avg, t.exp_avg_sq) == (state[i]["exp_avg"].data_ptr(), state[i]["exp_avg_sq"].data_ptr())
     assert {t.data_ptr() for st in opt._state.values() for t in st.values()}.isdisjoint(t.data_ptr() for st in twin._state.values() for t in st.values())
+
+
+def held(opt):
+    return ([(id(p), k, t.data_ptr(), t.clone()) for p, st in opt._state.items() for k, t in st.items()], [(d, t.tolist()) for d, t in opt._steps.items()],
+            [{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups])
+
+
+def same(a, b):
+    return all(x[:3] == y[:3] and torch.equal(x[3], y[3]) for x, y in zip(a[0], b[0])) and len(a[0]) == len(b[0]) and a[1:] == b[1:]
+
+
+@pytest.mark.parametrize("change", [
+    lambda sd: sd["state"][1].update(exp_avg=torch.zeros(8)), lambda sd: sd["state"][1].update(exp_avg_sq=None), lambda sd: sd["state"][1].pop("exp_avg_sq"),
+    lambda sd: sd["state"][1].pop("step"), lambda sd: sd["state"][1].update(step=float("nan")), lambda sd: sd["state"][1].update(step=-1),
+    lambda sd: sd["state"][1].update(step=2 ** 31), lambda sd: sd["state"].update({2: sd["state"][1]}), lambda sd: sd["state"].update({-1: sd["state"][1]}),
+    lambda sd: sd["state"].update({1: {"step": 1, "exp_avg": torch.zeros(7), "root": torch.zeros(7), "exp_avg_scale": torch.zeros(1), "root_scale": torch.zeros(1)}}),
+    lambda sd: sd["state"].update({1: {"step": 1, "exp_avg": torch.zeros(7, dtype=torch.uint8).view(torch.float8_e4m3fn), "exp_avg_scale": torch.zeros(1),
+                                       "root": torch.zeros(7, dtype=torch.uint8).view(torch.float8_e4m3fn), "root_scale": torch.zeros(2)}}),
+    lambda sd: sd["param_groups"][0].pop("betas"), lambda sd: sd["param_groups"][0].pop("lr"), lambda sd: sd["param_groups"][0].update(betas=(0.9, 1.0)),
+    lambda sd: sd["param_groups"][0].update(eps=-1.0), lambda sd: sd["param_groups"][0].update(weight_decay=-1.0), lambda sd: sd["param_groups"][0].update(amsgrad=True),
+    lambda sd: sd["param_groups"][0]["params"].pop(),
+])
+def test_a_refused_checkpoint_changes_nothing(monkeypatch, change):
+    """The optimiser goes on as one that was never asked: same moments at the same addresses, counts, groups, and the same next call."""
+    opt = stepped([torch.nn.Parameter(torch.zeros(4, 5)), torch.nn.Parameter(torch.zeros(7))])
+    bad = copy.deepcopy(opt.state_dict())
+    for st in bad["state"].values():
+        st["exp_avg"] += 1
+        st["step"] += 1
+    bad["param_groups"][0].update(lr=0.7, weight_decay=0.3)
+    change(bad)
+    before = held(opt)
+    with pytest.raises((ValueError, L.NndetError)):
+        opt.load_state_dict(bad)
+    assert same(before, held(opt))
+    calls = recorded(monkeypatch)
+    for p in opt.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert [(t.exp_avg, t.slot) for t in calls[0][1]] == [(opt._state[p]["exp_avg"].data_ptr(), i) for i, p in enumerate(opt.param_groups[0]["params"])]
