@@ -639,10 +639,10 @@ class AdamW:
                 if p in self._state:
                     st = dict(self._state[p])
                     if bits == 32 and "root" in st:
-                        full = torch.empty_like(p, dtype=torch.float32), torch.empty_like(p, dtype=torch.float32)
+                        full = [torch.empty_like(st["exp_avg"], dtype=torch.float32) for _ in range(2)]
                         read_adam_state8(AdamState8(*([st[k]] for k in AdamState8._fields)), [full[0]], [full[1]])
                         st = dict(zip(("exp_avg", "exp_avg_sq"), full))
-                    state[idx] = {"step": self._counts(p.device)[self._slot[p]].float(), **st}
+                    state[idx] = {"step": self._counts(st["exp_avg"].device)[self._slot[p]].float(), **st}
                 ids.append(idx); idx += 1
             groups.append({**{k: v for k, v in g.items() if k != "params"}, "amsgrad": False, "maximize": False, "foreach": None, "capturable": False,
                            "differentiable": False, "fused": None, "decoupled_weight_decay": True, "params": ids})

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from nndetection_amd import _lib as L
 from nndetection_amd import optim as O
 from tests.test_optim_gpu import BLOCK, DEV, U, check8, formula, gen, rows, within
 
@@ -52,3 +53,25 @@ def test_second_moments_below_the_normal_range(bits, eps, sizes):
             else:
                 within(m[i], *wm)
                 within(v[i], wv[0], ev)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_checkpoint_written_after_the_model_left_the_gpu(bits):
+    """model.cpu() before saving: the state lies where it lay, and its counts with it; back on the GPU the training goes on."""
+    net = torch.nn.Linear(40, 30).to(DEV)
+    opt = O.AdamW(net.parameters(), lr=0.1, state_bits=bits, min_8bit_numel=100)
+    for p in net.parameters():
+        p.grad = torch.ones_like(p)
+    for _ in range(3):
+        opt.step()
+    want = opt.state_dict(bits=32)
+    net.cpu()
+    got = opt.state_dict(bits=32)
+    for i in (0, 1):
+        assert float(got["state"][i]["step"]) == 3.0
+        assert all(torch.equal(got["state"][i][k], want["state"][i][k]) for k in ("exp_avg", "exp_avg_sq"))
+    with pytest.raises(L.NndetError, match="moved"):
+        opt.step()
+    net.to(DEV)
+    opt.step()
+    assert float(opt.state_dict()["state"][0]["step"]) == 4.0
