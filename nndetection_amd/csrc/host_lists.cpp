@@ -28,14 +28,14 @@ struct List {                                        // a list or tuple, or noth
 };
 
 // `o` as a plain dense GPU tensor on `device`, or nullptr
-const c10::TensorImpl* plain(const at::TensorBase& t, c10::DeviceIndex device) {
+c10::TensorImpl* plain(const at::TensorBase& t, c10::DeviceIndex device) {
     if (!t.defined()) return nullptr;
-    const c10::TensorImpl* x = t.unsafeGetTensorImpl();
+    c10::TensorImpl* x = t.unsafeGetTensorImpl();
     if (x->layout() != c10::kStrided || x->is_python_dispatch() || x->device() != c10::Device(c10::kCUDA, device)) return nullptr;
     if (!(x->is_contiguous() || x->is_non_overlapping_and_dense()) || (x->numel() && !x->data())) return nullptr;
     return x;
 }
-const c10::TensorImpl* plain(PyObject* o, c10::DeviceIndex device) {
+c10::TensorImpl* plain(PyObject* o, c10::DeviceIndex device) {
     return THPVariable_Check(o) ? plain(THPVariable_Unpack(o), device) : nullptr;
 }
 
@@ -75,7 +75,7 @@ struct Addresses {                                   // a set of addresses: open
 //   -> (structs, n) or None
 //   params None: grads alone. grads None: params[i].grad. A gradient that is None leaves its tensor out (slot = place in the list).
 //   exp_avgs None: no moments. bits: 32, 8, or 0 for either, by the type of exp_avgs[i]. weight_decay: a number or a list.
-//   both: grads are written too.
+//   both: grads are written too. What is written is taken by its mutable address, which gives a lazily cloned tensor memory of its own first.
 PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (nargs != 10) {
         PyErr_SetString(PyExc_TypeError, "pack() takes 10 arguments");
@@ -98,7 +98,7 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         Addresses seen((p.seq ? 1 + (both != 0) : 1) * n + (m.seq ? 2 * n : 0));
         Py_ssize_t k = 0;
         for (Py_ssize_t i = 0; i < n; ++i) {
-            const c10::TensorImpl *px = nullptr, *gx = nullptr;
+            c10::TensorImpl *px = nullptr, *gx = nullptr;
             if (g.seq && g[i] == Py_None) continue;
             if (p.seq) {
                 px = plain(p[i], device);
@@ -117,8 +117,8 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             const c10::TensorImpl* x = px ? px : gx;
             const int type = type_of(x);
             if (type < 0 || (px && (px->dtype() != gx->dtype() || !same(px, gx)))) goto other;
-            e.param = px ? const_cast<void*>(px->data()) : nullptr;
-            e.grad = const_cast<void*>(gx->data());
+            e.param = px ? px->mutable_data() : nullptr;
+            e.grad = both ? gx->mutable_data() : const_cast<void*>(gx->data());
             e.numel = x->numel();
             e.slot = (int32_t)i;
             e.dtype = (int16_t)type;
@@ -130,16 +130,16 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                 e.weight_decay = one_wd;
             }
             if (m.seq) {
-                const c10::TensorImpl *mx = plain(m[i], device), *vx = plain(v[i], device);
+                c10::TensorImpl *mx = plain(m[i], device), *vx = plain(v[i], device);
                 if (!mx || !vx || !same(mx, x) || !same(vx, x) || mx->dtype() != vx->dtype()) goto other;
-                e.exp_avg = const_cast<void*>(mx->data());
-                e.exp_avg_sq = const_cast<void*>(vx->data());
+                e.exp_avg = mx->mutable_data();
+                e.exp_avg_sq = vx->mutable_data();
                 if (is(mx, c10::ScalarType::Float8_e4m3fn) && bits != 32 && ms.seq) {
-                    const c10::TensorImpl *sx = plain(ms[i], device), *rx = plain(rs[i], device);
+                    c10::TensorImpl *sx = plain(ms[i], device), *rx = plain(rs[i], device);
                     const int64_t blocks = (e.numel + 255) / 256;
                     if (!sx || !rx || !is(sx, c10::ScalarType::Float) || !is(rx, c10::ScalarType::Float) || sx->numel() != blocks || rx->numel() != blocks) goto other;
-                    e.exp_avg_scale = (float*)const_cast<void*>(sx->data());
-                    e.root_scale = (float*)const_cast<void*>(rx->data());
+                    e.exp_avg_scale = (float*)sx->mutable_data();
+                    e.root_scale = (float*)rx->mutable_data();
                     e.state_bits = 8;
                 } else if (!is(mx, c10::ScalarType::Float) || bits == 8) {
                     goto other;

@@ -404,7 +404,7 @@ def adamw8_step(params, grads, state: AdamState8, steps: torch.Tensor, *, lr: Ra
 def _clip_call(grads, max_norm: float, grad_scale) -> torch.Tensor:
     n = len(grads)
     device = grads[0].device if n else torch.device("cuda", torch.cuda.current_device())
-    packed = _pack(device, None, grads, None, None, None, None, 0.0, 0)
+    packed = _pack(device, None, grads, None, None, None, None, 0.0, 0, max_norm >= 0.0)
     if packed is not None:
         norm = torch.empty((), dtype=torch.float32, device=device)
         _run(device, "nndet_grad_clip", *packed, max_norm, _scalar("grad_scale", grad_scale, device), norm.data_ptr())

@@ -75,3 +75,30 @@ def test_a_checkpoint_written_after_the_model_left_the_gpu(bits):
     net.to(DEV)
     opt.step()
     assert float(opt.state_dict()["state"][0]["step"]) == 4.0
+
+
+@pytest.mark.parametrize("listed", [True, False])
+def test_lazily_cloned_tensors_get_memory_of_their_own(listed):
+    """torch._lazy_clone shares the storage until one of the two is written: what a call writes must not reach the other. `listed` False: through
+    the Python checks (a gradient in another memory order)."""
+    g = gen(7)
+    mk = lambda: torch.randn(40, 60, generator=g, device=DEV)  # noqa: E731
+    first = {k: mk() for k in "pgm"} | {"v": mk().square()}
+    kept = {k: t.clone() for k, t in first.items()}
+    lazy = {k: torch._lazy_clone(t) for k, t in first.items()}
+    grad = lazy["g"] if listed else lazy["g"].t().contiguous().t()
+    steps = torch.zeros(1, dtype=torch.int32, device=DEV)
+    want = formula(first["p"], first["g"], first["m"], first["v"], 1, 1e-2, 0.9, 0.999, 1e-8, 0.01)
+    O.adamw_step([lazy["p"]], [grad], [lazy["m"]], [lazy["v"]], steps, lr=1e-2)
+    O.clip_grads_([lazy["g"]], 0.1)
+    assert all(torch.equal(first[k], kept[k]) for k in first)
+    for k, w in zip("pmv", want):
+        within(lazy[k], *w, what=k)
+    st = O.AdamState8.zeros([first["p"]])
+    m2, v2 = torch._lazy_clone(first["m"]), torch._lazy_clone(first["v"])
+    O.write_adam_state8(st, [m2], [v2])
+    lazy8 = O.AdamState8(*([torch._lazy_clone(t[0])] for t in st))
+    codes = [t[0].view(torch.uint8).clone() for t in st]
+    O.adamw8_step([lazy["p"]], [grad], lazy8, steps, lr=1e-2)
+    O.read_adam_state8(lazy8, [m2], [v2])
+    assert all(torch.equal(t[0].view(torch.uint8), c) for t, c in zip(st, codes)) and torch.equal(first["m"], kept["m"]) and torch.equal(first["v"], kept["v"])
