@@ -4,6 +4,7 @@ There is NO fallback: if the library is missing or a call fails, an exception is
 only used for device memory (caching allocator) and the current stream.
 """
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -462,6 +463,44 @@ if not PRIVATE_AUTOGRAD_HOOKS:
 def graph_task_id() -> int:
     """Id of the backward pass that is running on this thread, -1 outside of one (or when torch does not tell)."""
     return _graph_task_id() if _graph_task_id is not None else -1
+
+
+# Parameters that a captured optimiser step writes (AdamW): their version counters advance when the step is captured, not when it is replayed, and
+# no host code runs at a replay. Whatever is cached from such a parameter (arch/conv.py: _pver) is therefore keyed on a count that advances whenever
+# somebody asks for it from outside of a `fresh_params` call and of a backward pass, and once at the start of such a call.
+graph_written = {}                                   # address of a storage -> count
+_in_fresh_params = [False]
+
+
+def note_graph_write(tensors) -> None:
+    for t in tensors:
+        graph_written.setdefault(t.untyped_storage().data_ptr(), 0)
+
+
+def graph_write_count(t) -> int:
+    at = t.untyped_storage().data_ptr()
+    n = graph_written.get(at)
+    if n is None:
+        return 0
+    if not _in_fresh_params[0] and graph_task_id() == -1:
+        n = graph_written[at] = n + 1
+    return n
+
+
+def fresh_params(method):
+    """Decorator of a module's method: within a call, what is cached from a parameter that replays write is made once, from the values at its start."""
+    @functools.wraps(method)
+    def call(self, *args, **kwargs):
+        if not graph_written or _in_fresh_params[0]:
+            return method(self, *args, **kwargs)
+        for p in self.parameters():
+            graph_write_count(p)
+        _in_fresh_params[0] = True
+        try:
+            return method(self, *args, **kwargs)
+        finally:
+            _in_fresh_params[0] = False
+    return call
 
 
 _cumask_streams = []                                 # (keeps the raw handles alive for the life of the process)

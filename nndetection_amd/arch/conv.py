@@ -69,7 +69,8 @@ def bump_param_generation(*_args, **_kwargs) -> None:
 
 
 def _pver(t: torch.Tensor):
-    return (t._version, t.data_ptr(), PARAM_GENERATION[0])
+    ver = (t._version, t.data_ptr(), PARAM_GENERATION[0])
+    return ver + (L.graph_write_count(t),) if L.graph_written else ver
 
 
 # Caches that do not hang off a conv block (arch/pyramid.py: the packed weights of two FUSED blocks) are additionally keyed on this
@@ -166,7 +167,8 @@ def prepack_all(model: nn.Module, dtype: torch.dtype, modes=(0, 1), force: bool 
                 d.k = (ctypes.c_int32 * 3)(*mod.k); d.s = (ctypes.c_int32 * 3)(*mod.s); d.p = (ctypes.c_int32 * 3)(*mod.p)
                 job = mod._pack_cache[("job", mode, dtype)] = (d, int(L.load().nndet_packed_weight_elems(ctypes.byref(d), mode)))
             d, n = job
-            buf = hit[1] if (hit is not None and hit[1].numel() == n and hit[1].dtype == dtype and hit[1].device == w.device) else None
+            # (not in place where replays write parameters: such a buffer may have been packed on another stream, outside of this function)
+            buf = hit[1] if (hit is not None and not L.graph_written and hit[1].numel() == n and hit[1].dtype == dtype and hit[1].device == w.device) else None
             if buf is None:
                 buf = torch.empty((n,), dtype=dtype, device=w.device)
             w32 = w.detach()

@@ -145,6 +145,7 @@ class BaseRetinaNet(nn.Module):
                     torch.zeros(1, device=device)                # (first use)
 
     # ------------------------------------------------------------------ forward (retina.py:198-226)
+    @L.fresh_params
     def forward(self, inp: Tensor):
         if inp.is_cuda and BaseRetinaNet._bind_order:
             self._bind_streams(inp.device)
@@ -310,6 +311,7 @@ class BaseRetinaNet(nn.Module):
         return pool[i]
 
     # ------------------------------------------------------------------ train step (retina.py:86-159)
+    @L.fresh_params
     def train_step(self, images: Tensor, targets: dict, evaluation: bool, batch_num: int = 0):
         """`targets`: the reference's dict (target_boxes, target_classes, target_seg) or a `core.targets.DeferredTargets`, whose
         box lists become available on the host only after `resolve()`: then the forward pass is queued FIRST and the target

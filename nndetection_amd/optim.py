@@ -250,8 +250,8 @@ def _words(n, p, g, m, v, ms, rs, numel, wd, tail) -> bytes:
     return array.array("q", [w for row in rows for w in row]).tobytes()
 
 
-def _run(device, what: str, words, n: int, *args) -> None:
-    """Call `what`(tensors, n, *args, workspace, bytes, stream) on the device's current stream, with a workspace of this call."""
+def _run(device, what: str, words, n: int, *args) -> bool:
+    """Call `what`(tensors, n, *args, workspace, bytes, stream) on the device's current stream, with a workspace of this call. True if that is being captured."""
     if device.type != "cuda":
         _refuse(f"tensors on {device}: nndetection_amd kernels need tensors on the GPU (no CPU path)")
     if device.index != torch.cuda.current_device():
@@ -260,6 +260,7 @@ def _run(device, what: str, words, n: int, *args) -> None:
     nbytes = L.load().nndet_opt_workspace_bytes(n)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=device)
     L.call(what, words, n, *args, ws.data_ptr(), nbytes, L.stream())
+    return torch.cuda.is_current_stream_capturing()
 
 
 def _ptrs(ts) -> list:
@@ -333,7 +334,8 @@ def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight
     a, norm = _hyper(lr, betas, eps, max_norm, total_norm, grad_scale, found_inf, steps, steps.device)
     packed = _pack(steps.device, params, grads, m, v, ms, rs, weight_decay, bits)
     if packed is not None:
-        _run(steps.device, "nndet_adamw_step", *packed, L.C.byref(a))
+        if _run(steps.device, "nndet_adamw_step", *packed, L.C.byref(a)):
+            L.note_graph_write([p for p, g in zip(params, grads) if g is not None])
         L.host_lists().written(params, grads)
         return norm
     wd = weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
@@ -358,7 +360,8 @@ def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight
     bits_of = {w: _double_bits(float(w)) for w in set(wd)}
     words = _words(n, _ptrs(params), _ptrs(grads), _ptrs(m), _ptrs(v), ms and _ptrs(ms), rs and _ptrs(rs), numel, [bits_of[w] for w in wd],
                    [s | k | (bits << 48) for s, k in zip(slots, kinds)])
-    _run(device, "nndet_adamw_step", words, n, L.C.byref(a))
+    if _run(device, "nndet_adamw_step", words, n, L.C.byref(a)):
+        L.note_graph_write(params)
     _written(params)
     return norm
 
@@ -466,7 +469,8 @@ def _state8_call(state: AdamState8, exp_avgs, exp_avg_sqs, write: int) -> None:
     device = exp_avgs[0].device
     packed = _pack(device, exp_avgs, exp_avg_sqs, state.exp_avg, state.root, state.exp_avg_scale, state.root_scale, 0.0, 8, True)
     if packed is not None and exp_avgs[0].dtype == torch.float32:
-        return _run(device, "nndet_adam_state8", *packed, write)
+        _run(device, "nndet_adam_state8", *packed, write)
+        return
     _check_list("exp_avgs", exp_avgs, torch.float32, device)
     _check_list("exp_avg_sqs", exp_avg_sqs, torch.float32, device, exp_avgs)
     _check_list("exp_avg", state.exp_avg, _F8, device, exp_avgs)
@@ -507,7 +511,8 @@ class AdamW:
     max_norm: clip by the global gradient norm within the step (the gradients themselves are not written); `grad_norm` holds the norm of
     the last step, on the GPU.
     lr: a number, or one fp32 value on the GPU, which a captured step reads. A step can be captured once every parameter has a state, i.e.
-    after a first step outside of the capture."""
+    after a first step outside of the capture. What this package keeps of the parameters (packed weights) follows the replays; what other code keys on
+    a parameter's version counter does not see them."""
 
     _step_supports_amp_scaling = True                # torch.amp.GradScaler hands grad_scale / found_inf over as device tensors
 
@@ -581,8 +586,10 @@ class AdamW:
                     g = self.param_groups[0]
                     on = lambda t: None if t is None else t.to(device)  # noqa: E731
                     a, self.grad_norm = _hyper(g["lr"], g["betas"], g["eps"], self.max_norm, None, on(scale), on(found), counts, device)
-                    _run(device, "nndet_adamw_step", *packed, L.C.byref(a))
-                    _written(self._flat if packed[1] == len(self._flat) else [p for p in self._flat if p.grad is not None])
+                    ps = self._flat if packed[1] == len(self._flat) else [p for p in self._flat if p.grad is not None]
+                    if _run(device, "nndet_adamw_step", *packed, L.C.byref(a)):
+                        L.note_graph_write(ps)
+                    _written(ps)
                 return
         calls = {}
         for g in self.param_groups:
@@ -623,7 +630,8 @@ class AdamW:
             counts = self._counts(device)
             a, self.grad_norm = _hyper(g["lr"], g["betas"], g["eps"], self.max_norm, on(total, device), on(scale, device), on(found, device),
                                        counts, device)
-            _run(device, "nndet_adamw_step", array.array("q", words).tobytes(), len(ps), L.C.byref(a))
+            if _run(device, "nndet_adamw_step", array.array("q", words).tobytes(), len(ps), L.C.byref(a)):
+                L.note_graph_write(ps)
             _written(ps)
 
     # ---- checkpointing, laid out like torch.optim.AdamW.state_dict(). Parameters with 8-bit moments hold those of `AdamState8` in place of

@@ -102,3 +102,84 @@ def test_lazily_cloned_tensors_get_memory_of_their_own(listed):
     O.adamw8_step([lazy["p"]], [grad], lazy8, steps, lr=1e-2)
     O.read_adam_state8(lazy8, [m2], [v2])
     assert all(torch.equal(t[0].view(torch.uint8), c) for t, c in zip(st, codes)) and torch.equal(first["m"], kept["m"]) and torch.equal(first["v"], kept["v"])
+
+
+def capture_steps(opt):
+    opt.step()                                       # (the first step makes the state)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    return graph
+
+
+def random_grads(params, seed):
+    for i, p in enumerate(params):
+        p.grad = torch.randn(p.shape, generator=gen(seed + i), device=DEV)
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_a_conv_block_follows_replayed_steps(fast):
+    """The packed weights of a block used on its own, forward and backward, after each replay: those of a block that keeps none. `fast` False: two rates."""
+    from nndetection_amd.arch.conv import ConvInstanceRelu
+    torch.manual_seed(0)
+    mk = lambda: ConvInstanceRelu(3, 32, 32, 3, padding=1).to(DEV)  # noqa: E731
+    block, plain = mk(), mk()
+    ps = list(block.parameters())
+    opt = O.AdamW(ps if fast else [{"params": ps[:1], "lr": 0.2}, {"params": ps[1:], "lr": 0.1}], lr=0.2)
+    random_grads(ps, 3)
+    x = torch.randn(2, 32, 8, 8, 8, generator=gen(1), device=DEV)
+    up = torch.randn(2, 32, 8, 8, 8, generator=gen(2), device=DEV)
+
+    def both(net):
+        z = x.clone().requires_grad_()
+        y = net(z)
+        gx, = torch.autograd.grad(y, z, up)          # (the parameters' gradients stay what they are)
+        return y.detach(), gx
+
+    both(block)
+    graph = capture_steps(opt)
+    before = both(block)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        plain.load_state_dict(block.state_dict())
+        plain._pack_cache.clear()
+        got, want = both(block), both(plain)
+        for a, b, old in zip(got, want, before):
+            # the two run the same kernels on the same weights; only the order of fp64 sums of the norm may differ
+            assert float((a - b).abs().max()) <= 1e-5 * float(b.abs().max())
+            assert float((a - old).abs().max()) > 1e-2 * float(b.abs().max())
+        before = got
+        with torch.no_grad():
+            assert float((block(x) - want[0]).abs().max()) <= 1e-5 * float(want[0].abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_detector_in_evaluation_follows_replayed_steps(dtype):
+    from nndetection_amd.plans import get_plan
+    from nndetection_amd.ptmodule import build_model
+    from tests.gpu_util import synth_inputs
+    plan = get_plan("tiny")
+    torch.manual_seed(0)
+    net = build_model(plan).to(DEV).eval()
+    x = synth_inputs(plan)[0].to(DEV, dtype)
+    opt = O.AdamW(net.parameters(), lr=3e-2)
+    random_grads(net.parameters(), 5)
+    logits = lambda: torch.cat([t.float().flatten() for t in net(x)[0].values() if isinstance(t, torch.Tensor)])  # noqa: E731
+    probs = lambda: net.inference_step(x)["pred_seg"].float()  # noqa: E731
+    with torch.no_grad():
+        logits(), probs()
+        graph = capture_steps(opt)
+        old = logits(), probs()
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            got = logits(), probs()
+            net.train(), net.eval()                  # (drops everything that is kept of the parameters)
+            want = logits(), probs()
+            tol = 1e-4 if dtype == torch.float32 else 2e-2           # statistics are summed by atomics; 16 bits store their noise
+            for a, b, c in zip(got, want, old):
+                assert float((a - b).abs().max()) <= tol * float(b.abs().max())
+                assert float((a - c).abs().max()) > 3 * tol * float(b.abs().max())
+            old = got

@@ -89,3 +89,44 @@ def test_a_refused_checkpoint_changes_nothing(monkeypatch, change):
         p.grad = torch.ones_like(p)
     opt.step()
     assert [(t.exp_avg, t.slot) for t in calls[0][1]] == [(opt._state[p]["exp_avg"].data_ptr(), i) for i, p in enumerate(opt.param_groups[0]["params"])]
+
+
+def test_versions_of_parameters_that_replays_write(monkeypatch):
+    """Outside of a `fresh_params` call every look is another version; within one it is one version, another than before; in a backward pass the last."""
+    from nndetection_amd.arch.conv import _pver
+    monkeypatch.setattr(L, "graph_written", {})
+    net = torch.nn.Linear(3, 2)
+    w, b = net.weight, net.bias
+    assert _pver(w) == _pver(w)
+    L.note_graph_write([w.detach().view(-1)])        # (a view of the parameter: it is the storage that counts)
+    seen = [_pver(w) for _ in range(3)]
+    assert len(set(seen)) == 3 and _pver(b) == _pver(b)
+
+    class Net(torch.nn.Linear):
+        @L.fresh_params
+        def inner(self):
+            return _pver(w), _pver(w)
+
+        @L.fresh_params
+        def forward(self, x):
+            return [_pver(w), *self.inner(), _pver(w)]
+
+    outer = Net(3, 2)
+    outer.weight, outer.bias = w, b
+    first, second = outer(None), outer(None)
+    assert len(set(first)) == len(set(second)) == 1 and first[0] != second[0] and first[0] not in seen
+    looked = []
+
+    class F(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 1
+
+        @staticmethod
+        def backward(ctx, g):
+            looked.extend([_pver(w), _pver(w)])
+            return g
+
+    F.apply(torch.ones(1, requires_grad=True)).sum().backward()
+    assert looked == [second[0]] * 2
+    assert _pver(w) != second[0]
