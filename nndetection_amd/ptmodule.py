@@ -100,7 +100,8 @@ def configure_optimizer(model: nn.Module, trainer_cfg: dict = None, lean: bool =
     lean=True: the foreach-based implementation of nndetection_amd/optim.py (same arithmetic, far less host time);
     lean=False: torch.optim.SGD + LambdaLR.
     trainer_cfg["optimizer"] = "adamw" / "adamw8" (default "sgd"): AdamW on the same groups and schedule, with moments in 32 / 8 bits
-    (lean=False: torch.optim.AdamW); "adamw_betas", "adamw_eps" and "max_norm" (clipping within the step, lean only) go with it."""
+    (lean=False: torch.optim.AdamW, 32 bits); "adamw_betas", "adamw_eps" and "max_norm" (clipping within the step, lean only) go with it.
+    What the chosen optimiser cannot do is refused."""
     cfg = dict(TRAINER_CFG_V001 if trainer_cfg is None else trainer_cfg)
     groups = get_params_no_wd_on_norm(model, cfg["weight_decay"])
     total = cfg["max_num_epochs"] * cfg["num_train_batches_per_epoch"]
@@ -108,6 +109,10 @@ def configure_optimizer(model: nn.Module, trainer_cfg: dict = None, lean: bool =
     kind = cfg.get("optimizer", "sgd")
     if kind not in ("sgd", "adamw", "adamw8"):
         raise ValueError(f"trainer_cfg['optimizer'] = {kind!r}: 'sgd', 'adamw' or 'adamw8'")
+    if cfg.get("max_norm") is not None and (kind == "sgd" or not lean):
+        raise ValueError("trainer_cfg['max_norm'] clips within the step of the lean AdamW; for other optimisers call optim.clip_grad_norm_ before the step")
+    if kind == "adamw8" and not lean:
+        raise ValueError("trainer_cfg['optimizer'] = 'adamw8': torch.optim.AdamW (lean=False) has no moments in 8 bits")
     if kind != "sgd" and lean:
         from .optim import AdamW, LinearWarmupPolyLR
         opt = AdamW(groups, lr0, betas=cfg.get("adamw_betas", (0.9, 0.999)), eps=cfg.get("adamw_eps", 1e-8),
@@ -299,6 +304,10 @@ class RetinaUNetAMDSteps:
         """The reference's `configure_optimizers` (retinaunet/base.py:300-336: SGD + nesterov, no weight decay on norms,
         LinearWarmupPolyLR per iteration) unchanged, then `amd_fuse_sgd` on every torch.optim.SGD it returned."""
         parent = getattr(super(), "configure_optimizers", None)
+        cfg = getattr(self, "trainer_cfg", None) or {}
+        if parent is not None and (cfg.get("optimizer", "sgd") != "sgd" or cfg.get("max_norm") is not None):
+            raise ValueError("trainer_cfg['optimizer'] / ['max_norm']: the registered module trains with the reference's configure_optimizers (SGD); AdamW is "
+                             "what StandaloneRetinaUNetV001AMD and ptmodule.configure_optimizer build")
         res = parent() if parent is not None else configure_optimizer(self.model, getattr(self, "trainer_cfg", None), lean=True)
         opts = res[0] if isinstance(res, (tuple, list)) and res and isinstance(res[0], (tuple, list)) else [res]
         for o in opts:

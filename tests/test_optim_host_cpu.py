@@ -130,3 +130,33 @@ def test_versions_of_parameters_that_replays_write(monkeypatch):
     F.apply(torch.ones(1, requires_grad=True)).sum().backward()
     assert looked == [second[0]] * 2
     assert _pver(w) != second[0]
+
+
+def test_requests_that_an_optimiser_cannot_keep_are_refused():
+    from nndetection_amd.plans import TRAINER_CFG_V001, get_plan
+    from nndetection_amd.ptmodule import RetinaUNetAMDSteps, StandaloneRetinaUNetV001AMD, build_model, configure_optimizer
+    m = build_model(get_plan("tiny"))
+    for kw, lean, match in ((dict(max_norm=12.0), True, "max_norm"), (dict(max_norm=12.0), False, "max_norm"), (dict(optimizer="adamw", max_norm=1.0), False, "max_norm"),
+                            (dict(optimizer="adamw8"), False, "8 bits")):
+        with pytest.raises(ValueError, match=match):
+            configure_optimizer(m, dict(TRAINER_CFG_V001, **kw), lean=lean)
+    assert isinstance(configure_optimizer(m, dict(TRAINER_CFG_V001, max_norm=None), lean=False)[0], torch.optim.SGD)
+
+    class Reference:                                 # (what the registered module inherits from: SGD, whatever the configuration says)
+        def configure_optimizers(self):
+            return [torch.optim.SGD(self.model.parameters(), 0.1)], []
+
+    class Registered(RetinaUNetAMDSteps, Reference):
+        pass
+
+    module = Registered.__new__(Registered)
+    module.model = m
+    for cfg, ok in ((None, True), ({}, True), (dict(TRAINER_CFG_V001), True), (dict(optimizer="sgd", max_norm=None), True), (dict(optimizer="adamw"), False),
+                    (dict(optimizer="adamw8"), False), (dict(max_norm=12.0), False)):
+        module.trainer_cfg = cfg
+        if ok:
+            assert isinstance(module.configure_optimizers()[0][0], torch.optim.SGD)
+        else:
+            with pytest.raises(ValueError, match="StandaloneRetinaUNetV001AMD"):
+                module.configure_optimizers()
+    assert StandaloneRetinaUNetV001AMD is not None
