@@ -2,7 +2,7 @@
 // conversion between fp32 and 8-bit moments.
 //
 // A call takes n tensors of any sizes. k_opt_table copies their addresses out of the kernel arguments into a table in the workspace (64 B
-// a tensor, up to 99 of them a launch (166 gradients), so that every later kernel is ONE launch whatever n is), advances the step counts and works out what
+// a tensor, up to 99 of them a launch (164 gradients), so that every later kernel is ONE launch whatever n is), advances the step counts and works out what
 // is the same for a whole tensor. Then one launch per storage kind (type of the parameters x bits of the moments) has a workgroup for each
 // tile of 2048 consecutive elements of a tensor; no tile spans two tensors. A wave owns blocks of 256 consecutive elements, which are also
 // the blocks that share a scale of the 8-bit moments: the maximum never leaves the wave. Calls of few small tensors skip the table,
@@ -66,14 +66,20 @@ struct OptHead { float factor; int32_t skip; int32_t pad[14]; };
 // A tensor in the kernel arguments: its PTRS addresses (48 bits each; 1: grad, 4: param, grad, moments, 6: and the scales), numel below 2^40, slot.
 template <int PTRS> struct OptArg { uint32_t lo[PTRS]; uint16_t hi[PTRS]; uint32_t numel_lo, numel_hi_slot; float wd; uint32_t tile0; };
 template <int PTRS> struct OptTableArgs {
-    static constexpr int MOST = PTRS == 1 ? 166 : PTRS == 4 ? 99 : 76;     // tensors a launch: what 4 KB of kernel arguments hold
+    static constexpr int MOST = PTRS == 1 ? 164 : PTRS == 4 ? 99 : 76;     // tensors a launch: what OPT_ARGS holds besides a kernel's other arguments
     OptHead* head; OptEntry* entry; OptCoef* coef; uint32_t* tile0; int32_t* steps;
     const float* lr_ptr; const float* found_inf; const float* grad_scale;
     double lr, log2_b1, log2_b2;
     int32_t n, first;                                    // tensors of this launch; first: it also writes the head
     OptArg<PTRS> a[MOST];
 };
-static_assert(sizeof(OptTableArgs<1>) <= 4096 && sizeof(OptTableArgs<4>) <= 4096 && sizeof(OptTableArgs<6>) <= 4096, "kernel arguments are limited to 4 KB");
+// Bytes of a kernel's arguments in their order. All kernels here keep to 4 KB, the size that kernel arguments can be relied on to have.
+static constexpr size_t OPT_ARGS = 4096;
+template <typename... T> constexpr size_t opt_args_bytes() {
+    size_t n = 0;
+    ((n = (n + alignof(T) - 1) / alignof(T) * alignof(T) + sizeof(T)), ...);
+    return n;
+}
 
 // After 16-byte stores, with all arithmetic before them (a sched_barrier): nothing may overwrite a store's data registers in its next slots
 // (tools/scan_store_hazard.py).
@@ -126,7 +132,10 @@ template <int PTRS> __device__ __forceinline__ void opt_write_table(const OptTab
     opt_stored();
 }
 template <int PTRS>
-__global__ __launch_bounds__(192) void k_opt_table(const OptTableArgs<PTRS> A) { opt_write_table(A, threadIdx.x); }
+__global__ __launch_bounds__(192) void k_opt_table(const OptTableArgs<PTRS> A) {
+    static_assert(opt_args_bytes<OptTableArgs<PTRS>>() <= OPT_ARGS && OptTableArgs<PTRS>::MOST <= 192, "arguments; a thread a tensor");
+    opt_write_table(A, threadIdx.x);
+}
 
 // The table is written by an earlier kernel and constant in this one: read it through the scalar cache, so that what is uniform for a
 // workgroup stays in scalar registers (the compiler cannot see that the kernel's own stores do not touch it).
@@ -505,6 +514,7 @@ __global__ __launch_bounds__(OPT_WG) void k_opt_sumsq(OptMem src, uint32_t tiles
 // The same with the tensors in the kernel arguments. A step (PTRS > 1) needs the table in the kernel behind: a workgroup of its own, the last, writes it.
 template <typename T, int NB, int PTRS>
 __global__ __launch_bounds__(OPT_WG) void k_opt_sumsq_own(const OptTableArgs<PTRS> A, uint32_t tiles, double* partial) {
+    static_assert(opt_args_bytes<OptTableArgs<PTRS>, uint32_t, double*>() <= OPT_ARGS && OptTableArgs<PTRS>::MOST <= (PTRS > 1 ? OPT_WG : 1 << 30), "arguments; a thread a tensor");
     const uint32_t wgs = gridDim.x - (PTRS > 1);
     if (PTRS > 1 && blockIdx.x == wgs) opt_write_table(A, threadIdx.x);
     else opt_sumsq_walk<T, NB>(OptOwn<PTRS>{A, A.n}, tiles, wgs, partial);
@@ -553,6 +563,7 @@ template <typename T>
 __global__ __launch_bounds__(OPT_WG) void k_opt_scale(OptMem src, uint32_t tiles, const OptHead* head, OptSums N) { opt_scale_walk<T>(src, tiles, head, N); }
 template <typename T>
 __global__ __launch_bounds__(OPT_WG) void k_opt_scale_own(const OptTableArgs<1> A, uint32_t tiles, OptSums N) {
+    static_assert(opt_args_bytes<OptTableArgs<1>, uint32_t, OptSums>() <= OPT_ARGS, "arguments");
     opt_scale_walk<T>(OptOwn<1>{A, A.n}, tiles, A.head, N);
 }
 
@@ -595,6 +606,7 @@ __global__ __launch_bounds__(OPT_WG) void k_opt_state8(OptMem src, uint32_t tile
 // host time and 2 - 4 us of GPU time, which is what such a call consists of.
 template <typename T, int BITS>
 __global__ __launch_bounds__(OPT_FEW_WG) void k_adamw_few(const OptTableArgs<BITS == 8 ? 6 : 4> A, OptHyper H, int clipped) {
+    static_assert(opt_args_bytes<OptTableArgs<BITS == 8 ? 6 : 4>, OptHyper, int>() <= OPT_ARGS, "arguments");
     if (opt_skip(A)) return;
     const OptEntry e = opt_entry(A.a[blockIdx.x]);
     const uint32_t slot = A.a[blockIdx.x].numel_hi_slot >> 8;
@@ -614,6 +626,7 @@ __global__ __launch_bounds__(OPT_FEW_WG) void k_adamw_few(const OptTableArgs<BIT
 // The norm of all tensors of the call by one workgroup, a wave a tensor; SCALE: and the gradients multiplied by the factor.
 template <typename T, bool SCALE, int PTRS>
 __global__ __launch_bounds__(OPT_FEW_WG) void k_opt_norm_few(const OptTableArgs<PTRS> A, double max_norm, float* norm_at) {
+    static_assert(opt_args_bytes<OptTableArgs<PTRS>, double, float*>() <= OPT_ARGS, "arguments");
     __shared__ double part[OPT_FEW_WG / 64];
     __shared__ float all;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
