@@ -7,7 +7,7 @@ import torch
 
 from nndetection_amd import _lib as L
 from nndetection_amd import optim as O
-from tests.test_optim_gpu import BLOCK, DEV, U, check8, formula, gen, rows, within
+from tests.test_optim_gpu import DEV, U, check8, formula, gen, guards_intact, make, rows, within, test_norm_and_clip as norm_and_clip
 
 pytestmark = pytest.mark.gpu
 TINY = 2.0 ** -149                                   # one denormal step
@@ -183,3 +183,103 @@ def test_a_detector_in_evaluation_follows_replayed_steps(dtype):
                 assert float((a - b).abs().max()) <= tol * float(b.abs().max())
                 assert float((a - c).abs().max()) > 3 * tol * float(b.abs().max())
             old = got
+
+
+def many(n, big=9000):
+    """n sizes, most of them small, some empty: at the ends, and around every 256th place (a look-up reads 256 tensors at a time)."""
+    sizes = [1 + (37 * i * i) % 600 for i in range(n)]
+    for i in range(n):
+        if i % 256 in (0, 255) and i % 512 or i % 50 == 7 or i == n - 1:
+            sizes[i] = 0
+    sizes[3] = big                                   # (not a call of few small tensors)
+    sizes[n - 2] = 2500                              # two tiles behind the last round's boundary
+    return sizes
+
+
+@pytest.mark.parametrize("n", [99, 100, 255, 256, 257, 600])
+@pytest.mark.parametrize("clip,dtype", [(False, torch.float32), (True, torch.float32), (True, torch.bfloat16)])
+def test_a_step_of_many_tensors_of_one_kind(n, clip, dtype):
+    """Around what one launch's arguments hold (99), what a round of the tensor look-up reads (256), and several launches. Each tensor has its own count and decay."""
+    x = make(many(n), dtype, seed=n)
+    steps = torch.arange(n, dtype=torch.int32, device=DEV)
+    wd = [0.1 * (i % 4) for i in range(n)]
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in x["g"]))
+    factor = 0.5 * norm / (norm + 1e-6) if clip else 1.0
+    want = [formula(p, g, m, v, i + 1, 3e-3, 0.9, 0.999, 1e-8, wd[i], factor) for i, (p, g, m, v) in enumerate(zip(*(x[k] for k in "pgmv")))]
+    got = O.adamw_step(x["p"], x["g"], x["m"], x["v"], steps, lr=3e-3, weight_decay=wd, max_norm=0.5 * norm if clip else None)
+    assert got is None if not clip else abs(float(got) - norm) <= 2 * U * norm
+    assert torch.equal(steps, torch.arange(1, n + 1, dtype=torch.int32, device=DEV))
+    for i, (wp, wm, wv) in enumerate(want):          # (clipped: the norm's and the factor's rounding, as in the tests of few tensors)
+        within(x["p"][i], wp[0], 1.5 * wp[1], dtype, f"p {i}")
+        within(x["m"][i], wm[0], 1.5 * wm[1], what=f"m {i}")
+        within(x["v"][i], wv[0], 1.5 * wv[1], what=f"v {i}")
+    assert all(guards_intact(v, b, 0) for v, b in x["buf"])
+
+
+@pytest.mark.parametrize("n", [76, 77, 256, 257, 600])
+@pytest.mark.parametrize("clip,dtype", [(False, torch.float32), (True, torch.float32), (True, torch.float16)])
+def test_an_8_bit_step_of_many_tensors_of_one_kind(n, clip, dtype):
+    """The same with 8-bit moments (76 tensors a launch), written and read back on the way."""
+    sizes = many(n)
+    x = make(sizes, dtype, seed=1000 + n)
+    st = O.AdamState8.zeros(x["p"])
+    O.write_adam_state8(st, x["m"], x["v"])
+    for i, k in enumerate(sizes):
+        if k:
+            r = x["v"][i].double().sqrt()
+            check8(st, i, x["m"][i].double(), torch.zeros_like(r), r, U * r + TINY, True)
+    m0, v0 = [torch.empty_like(t) for t in x["m"]], [torch.empty_like(t) for t in x["v"]]
+    O.read_adam_state8(st, m0, v0)
+    for i, k in enumerate(sizes):
+        m = (rows(st.exp_avg[i].float()) * st.exp_avg_scale[i].view(-1, 1)).view(-1)[:k]
+        r = (rows(st.root[i].float()) * st.root_scale[i].view(-1, 1)).view(-1)[:k]
+        assert torch.equal(m0[i], m) and torch.equal(v0[i], r * r)
+    steps = torch.arange(n, dtype=torch.int32, device=DEV)
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in x["g"]))
+    factor = 0.5 * norm / (norm + 1e-6) if clip else 1.0
+    want = [formula(p, g, m, v, i + 1, 3e-3, 0.9, 0.999, 1e-8, 0.1, factor) for i, (p, g, m, v) in enumerate(zip(x["p"], x["g"], m0, v0))]
+    got = O.adamw8_step(x["p"], x["g"], st, steps, lr=3e-3, weight_decay=0.1, max_norm=0.5 * norm if clip else None)
+    assert got is None if not clip else abs(float(got) - norm) <= 2 * U * norm
+    assert torch.equal(steps, torch.arange(1, n + 1, dtype=torch.int32, device=DEV))
+    for i, (wp, wm, wv) in enumerate(want):
+        if sizes[i]:
+            within(x["p"][i], wp[0], 2 * wp[1], dtype, f"p {i}")
+            r = wv[0].sqrt()
+            check8(st, i, wm[0], 2 * wm[1], r, 8 * U * r + 2.0 ** -74, False)
+    assert all(guards_intact(v, b, 0) for v, b in x["buf"])
+
+
+@pytest.mark.parametrize("n", [164, 165, 256, 257, 600])
+@pytest.mark.parametrize("big", [9000, 300])
+def test_clipping_of_many_tensors_of_one_type(n, big):
+    """Around what one launch's arguments hold (164), with and without the kernel for few small tensors. (test_norm_and_clip adds two tensors.)"""
+    for dtype in (torch.float32, torch.bfloat16):
+        norm_and_clip(dtype, 1, many(n, big))
+        norm_and_clip(dtype, 0, many(n - 2, big))
+
+
+@pytest.mark.parametrize("clip", [False, True])
+def test_an_optimizer_of_both_kinds_of_moments_with_many_tensors(clip):
+    """AdamW(state_bits=8) with 120 parameters that keep 32 bits and 90 that do not: two tables of two launches each, two sums and two steps."""
+    shapes = [(1 + i % 97,) if i % 7 < 4 else (64, 64 + i % 5) for i in range(210)]
+    g = gen(11)
+    ps = [torch.nn.Parameter(torch.randn(s, generator=g, device=DEV)) for s in shapes]
+    random_grads(ps, 700)
+    norm = math.sqrt(sum(float(p.grad.double().square().sum()) for p in ps))
+    opt = O.AdamW([{"params": ps[::2], "weight_decay": 0.1}, {"params": ps[1::2], "weight_decay": 0.0}], lr=1e-2, state_bits=8, max_norm=0.5 * norm if clip else None)
+    factor = 0.5 * norm / (norm + 1e-6) if clip else 1.0
+    for t in (1, 2):
+        old = [torch.zeros_like(p) for p in ps], [torch.zeros_like(p) for p in ps]
+        if t == 2:
+            full = opt.state_dict(bits=32)["state"]
+            order = [*range(0, 210, 2), *range(1, 210, 2)]
+            for i, st in full.items():
+                old[0][order[i]], old[1][order[i]] = st["exp_avg"], st["exp_avg_sq"]
+        want = [formula(p.detach(), p.grad, m, v, t, 1e-2, 0.9, 0.999, 1e-8, 0.0 if i % 2 else 0.1, factor) for i, (p, m, v) in enumerate(zip(ps, *old))]
+        opt.step()
+        for i, (p, w) in enumerate(zip(ps, want)):
+            within(p.detach(), w[0][0], 2 * w[0][1], what=f"{i} step {t}")
+        if clip:
+            assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+    kinds = [("root" in st) for st in opt.state_dict()["state"].values()]
+    assert sum(kinds) == 90 and len(kinds) == 210
