@@ -180,17 +180,26 @@ _host_lists = None
 
 
 def host_lists():
-    """The module csrc/nndet_host.so (built with the library): lists of tensors to the structs of an optimiser call."""
+    """The module csrc/nndet_host.so (built with the library): lists of tensors to the structs of an optimiser call. It reads torch's tensors where
+    the headers that it was compiled with say, so it is refused under any other torch or Python."""
     global _host_lists
     if _host_lists is None:
         import importlib.machinery
         import importlib.util
+        import sysconfig
         path = os.path.join(_HERE, "csrc", "nndet_host.so")
         if not os.path.isfile(path):
             raise NndetError(f"{path} not found: build it with nndetection_amd/csrc/build.sh")
         spec = importlib.util.spec_from_loader("nndet_host", importlib.machinery.ExtensionFileLoader("nndet_host", path))
-        _host_lists = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_host_lists)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise NndetError(f"{path} does not load ({e}): build it again with nndetection_amd/csrc/build.sh")
+        here = f"{torch.__version__} {sysconfig.get_config_var('SOABI')}"
+        if getattr(module, "built_for", None) != here:
+            raise NndetError(f"{path} was built for torch and Python {getattr(module, 'built_for', 'unknown')}, not {here}: build it again with nndetection_amd/csrc/build.sh")
+        _host_lists = module
     return _host_lists
 
 

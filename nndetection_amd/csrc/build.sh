@@ -47,12 +47,17 @@ build sparse_out.hip
 build segbranch.hip
 build optim.hip -ffp-contract=off
 build api.hip
-# the host side of the optimiser's tensor lists (torch's C++ headers; a Python module, no GPU code)
-if [ -z "$ASM_DIR" ] && { [ -n "$REBUILD" ] || [ ! -f nndet_host.so ] || [ build.sh -nt nndet_host.so ] || [ host_lists.cpp -nt nndet_host.so ] || [ ../../include/nndet_amd.h -nt nndet_host.so ]; }; then
-  read -r PYINC TORCH ABI < <(${PYTHON:-python3} -c "import sysconfig, os, torch; print(sysconfig.get_paths()['include'], os.path.dirname(torch.__file__), int(torch._C._GLIBCXX_USE_CXX11_ABI))")
-  g++ -O2 -std=c++17 -fPIC -shared -D_GLIBCXX_USE_CXX11_ABI=$ABI -I"$PYINC" -isystem "$TORCH/include" -isystem "$TORCH/include/torch/csrc/api/include" \
-    host_lists.cpp -o nndet_host.so -L"$TORCH/lib" -ltorch_python -ltorch_cpu -lc10 -Wl,-rpath,"$TORCH/lib" &
-  pids+=($!)
+# the host side of the optimiser's tensor lists (torch's C++ headers; a Python module, no GPU code). It has the layout of torch's tensors built in:
+# another torch or Python than it was built for compiles it again here, and _lib.host_lists() refuses it.
+if [ -z "$ASM_DIR" ]; then
+  HOST=$(${PYTHON:-python3} -c "import sysconfig, os, torch; print(sysconfig.get_paths()['include'], os.path.dirname(torch.__file__), int(torch._C._GLIBCXX_USE_CXX11_ABI), torch.__version__, sysconfig.get_config_var('SOABI'))")
+  read -r PYINC TORCH ABI VERSION SOABI <<< "$HOST"
+  if [ -n "$REBUILD" ] || [ ! -f nndet_host.so ] || [ "$(cat _obj/host_for 2>/dev/null)" != "$HOST" ] || [ build.sh -nt nndet_host.so ] || [ host_lists.cpp -nt nndet_host.so ] || [ ../../include/nndet_amd.h -nt nndet_host.so ]; then
+    rm -f _obj/host_for
+    g++ -O2 -std=c++17 -fPIC -shared -D_GLIBCXX_USE_CXX11_ABI=$ABI -DNNDET_BUILT_FOR="\"$VERSION $SOABI\"" -I"$PYINC" -isystem "$TORCH/include" -isystem "$TORCH/include/torch/csrc/api/include" \
+      host_lists.cpp -o nndet_host.so -L"$TORCH/lib" -ltorch_python -ltorch_cpu -lc10 -Wl,-rpath,"$TORCH/lib" && echo "$HOST" > _obj/host_for &
+    pids+=($!)
+  fi
 fi
 rc=0
 for p in "${pids[@]}"; do wait $p || rc=1; done

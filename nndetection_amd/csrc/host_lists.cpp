@@ -191,4 +191,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "nndet_host", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_nndet_host() { return PyModule_Create(&module); }
+// built_for: the torch and the Python whose headers this was compiled with (build.sh), which the loader compares with those that run
+PyMODINIT_FUNC PyInit_nndet_host() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", NNDET_BUILT_FOR) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

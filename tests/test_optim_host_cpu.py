@@ -160,3 +160,12 @@ def test_requests_that_an_optimiser_cannot_keep_are_refused():
             with pytest.raises(ValueError, match="StandaloneRetinaUNetV001AMD"):
                 module.configure_optimizers()
     assert StandaloneRetinaUNetV001AMD is not None
+
+
+def test_the_host_module_is_refused_under_another_torch(monkeypatch):
+    assert L.host_lists().built_for.split()[0] == torch.__version__
+    monkeypatch.setattr(L, "_host_lists", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    with pytest.raises(L.NndetError, match="built for torch and Python .* not 1.0.0"):
+        L.host_lists()
+    assert L._host_lists is None
