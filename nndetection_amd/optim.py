@@ -509,7 +509,7 @@ class AdamW:
     state_bits: 32, or 8 (2 bytes an element for both moments instead of 8); a parameter of fewer than `min_8bit_numel` elements keeps 32
     bits: it would not save anything, and norms and biases have few elements that share a block's scale.
     max_norm: clip by the global gradient norm within the step (the gradients themselves are not written); `grad_norm` holds the norm of
-    the last step, on the GPU.
+    the last step, on the GPU (None: no parameter had a gradient).
     lr: a number, or one fp32 value on the GPU, which a captured step reads. A step can be captured once every parameter has a state, i.e.
     after a first step outside of the capture. What this package keeps of the parameters (packed weights) follows the replays; what other code keys on
     a parameter's version counter does not see them."""
@@ -576,6 +576,7 @@ class AdamW:
     @torch.no_grad()
     def step(self) -> None:
         scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        self.grad_norm = None
         keys = {(id(g["lr"]) if isinstance(g["lr"], torch.Tensor) else g["lr"], *g["betas"], g["eps"]) for g in self.param_groups}
         if len(keys) == 1 and len(self._steps) == 1:         # one call; None if a state is missing or anything is out of the ordinary
             (device, counts), = self._steps.items()

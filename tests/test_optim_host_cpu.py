@@ -169,3 +169,10 @@ def test_the_host_module_is_refused_under_another_torch(monkeypatch):
     with pytest.raises(L.NndetError, match="built for torch and Python .* not 1.0.0"):
         L.host_lists()
     assert L._host_lists is None
+
+
+def test_a_step_without_gradients_has_no_norm():
+    opt = stepped([torch.nn.Parameter(torch.zeros(4, 5))], max_norm=1.0)
+    opt.grad_norm = torch.tensor(3.0)                # (of an earlier step)
+    opt.step()
+    assert opt.grad_norm is None
