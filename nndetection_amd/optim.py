@@ -170,7 +170,9 @@ class AdamState8(NamedTuple):
 
 
 def _dense(t: torch.Tensor) -> bool:
-    """Do the elements fill one piece of memory, in any order of the dimensions, each place once?"""
+    """Do the elements fill one piece of memory, in any order of the dimensions, each place once, as they are (no negation that is still to come)?"""
+    if t.is_neg():
+        return False
     if t.is_contiguous():
         return True
     size = 1
@@ -201,7 +203,7 @@ def _check_list(name: str, ts, dtype, device, like=None) -> None:
             p = like[i]
             if t.shape != p.shape:
                 _refuse(f"{name}[{i}] has shape {tuple(t.shape)}, the parameter {tuple(p.shape)}")
-            if not (t.is_contiguous() and p.is_contiguous()) and not (_dense(t) and _same_order(t, p)):
+            if not (_dense(t) and (t.is_contiguous() and p.is_contiguous() or _same_order(t, p))):
                 _refuse(f"{name}[{i}] has strides {t.stride()}, the parameter {p.stride()}: moments lie in the parameter's memory order")
         elif not _dense(t):
             _refuse(f"{name}[{i}] with strides {t.stride()} is not dense in memory")
@@ -223,7 +225,7 @@ def _scalar(name: str, t, device) -> Optional[int]:
     """Address of a one-element fp32 tensor on `device`, None for None."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device or t.is_neg():
         _refuse(f"{name} is one fp32 value on {device}")
     return t.data_ptr()
 
@@ -286,7 +288,7 @@ def _grads_like(params, grads) -> list:
             _refuse(f"grads[{i}] is {'sparse' if g.layout != torch.strided else 'of shape %s' % (tuple(g.shape),)}, the parameter is dense {tuple(p.shape)}")
         if g.dtype != p.dtype or g.device != p.device:
             _refuse(f"grads[{i}] is {g.dtype} on {g.device}, the parameter {p.dtype} on {p.device}")
-        if not (g.is_contiguous() and p.is_contiguous()) and not (_dense(g) and _same_order(g, p)):
+        if not (_dense(g) and (g.is_contiguous() and p.is_contiguous() or _same_order(g, p))):
             g = torch.empty_like(p).copy_(g.detach())
         out.append(g)
     return out
@@ -368,7 +370,7 @@ def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight
 
 def _check_scales(name: str, ts, numel, device) -> None:
     for i, (t, n) in enumerate(zip(ts, numel)):
-        if t.dtype != torch.float32 or t.device != device or t.numel() != -(-n // STATE8_BLOCK) or not t.is_contiguous():
+        if t.dtype != torch.float32 or t.device != device or t.numel() != -(-n // STATE8_BLOCK) or not t.is_contiguous() or t.is_neg():
             _refuse(f"{name}[{i}] is one fp32 value on {device} for each {STATE8_BLOCK} elements of the tensor ({-(-n // STATE8_BLOCK)}), contiguous")
 
 
@@ -418,7 +420,7 @@ def _clip_call(grads, max_norm: float, grad_scale) -> torch.Tensor:
         if g.layout != torch.strided:
             _refuse(f"grads[{i}] is sparse")
     kinds = _kinds(grads)
-    flat = [g if _dense(g) else g.contiguous() for g in grads]
+    flat = [g if _dense(g) else g.resolve_neg().contiguous() for g in grads]
     _check_list("grads", flat, None, device)
     if max_norm >= 0.0:
         _check_distinct("grads", grads)
@@ -605,7 +607,7 @@ class AdamW:
                 slot = self._slot[p]
                 m, v, ms, rs = (ts[slot] for ts in self._lists)
                 device = m.device
-                if p.device != device or p.shape != m.shape or (p.stride() != m.stride() and not (_dense(p) and _same_order(p, m))):
+                if p.device != device or p.shape != m.shape or p.is_neg() or (p.stride() != m.stride() and not (_dense(p) and _same_order(p, m))):
                     _refuse(f"a parameter of shape {tuple(p.shape)} on {p.device} was moved or changed its size after its state was made")
                 # (its type may have changed: the moments are fp32 or 8 bits whatever it is)
                 tail = slot | _kinds([p])[0] | ((32 if ms is None else 8) << 48)

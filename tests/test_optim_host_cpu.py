@@ -176,3 +176,23 @@ def test_a_step_without_gradients_has_no_norm():
     opt.grad_norm = torch.tensor(3.0)                # (of an earlier step)
     opt.step()
     assert opt.grad_norm is None
+
+
+def test_tensors_with_a_negation_to_come(monkeypatch):
+    """torch's lazy negation (the imaginary part of a conjugate): a gradient is taken with its sign, what would be written is refused."""
+    seen = []
+    monkeypatch.setattr(O, "_run", lambda device, what, words, n, *args: seen.append(
+        [(C.c_float * t.numel).from_address(t.grad)[:] for t in (L.NndetOptTensor * n).from_buffer_copy(words)]))
+    mk = lambda *v: torch._neg_view(torch.tensor(v))  # noqa: E731
+    p, m, v, steps = torch.zeros(3), torch.zeros(3), torch.zeros(3), torch.zeros(1, dtype=torch.int32)
+    O.adamw_step([p], [mk(1.0, 2.0, 3.0)], [m], [v], steps, lr=0.1)
+    O.clip_grads_([mk(1.0, 2.0, 3.0)], 1.0)
+    O.grad_norm([mk(4.0, 5.0), torch.conj(torch.complex(torch.zeros(1), torch.ones(1))).imag])
+    assert seen == [[[-1.0, -2.0, -3.0]], [[-1.0, -2.0, -3.0]], [[-4.0, -5.0], [-1.0]]]
+    g = torch.ones(3)
+    for a in (([mk(0.0, 0.0, 0.0)], [g], [m], [v]), ([p], [g], [mk(0.0, 0.0, 0.0)], [v]), ([p], [g], [m], [mk(0.0, 0.0, 0.0)])):
+        with pytest.raises(L.NndetError):
+            O.adamw_step(*a, steps, lr=0.1)
+    with pytest.raises(L.NndetError, match="grad_scale"):
+        O.adamw_step([p], [g], [m], [v], steps, lr=0.1, grad_scale=mk(-2.0)[0])
+    assert len(seen) == 3
