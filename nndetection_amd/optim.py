@@ -469,10 +469,11 @@ def _state8_call(state: AdamState8, exp_avgs, exp_avg_sqs, write: int) -> None:
     if n == 0:
         return
     device = exp_avgs[0].device
+    out = [t for ts in state for t in ts] if write else [*exp_avgs, *exp_avg_sqs]
     packed = _pack(device, exp_avgs, exp_avg_sqs, state.exp_avg, state.root, state.exp_avg_scale, state.root_scale, 0.0, 8, True)
     if packed is not None and exp_avgs[0].dtype == torch.float32:
         _run(device, "nndet_adam_state8", *packed, write)
-        return
+        return _written(out)
     _check_list("exp_avgs", exp_avgs, torch.float32, device)
     _check_list("exp_avg_sqs", exp_avg_sqs, torch.float32, device, exp_avgs)
     _check_list("exp_avg", state.exp_avg, _F8, device, exp_avgs)
@@ -484,6 +485,7 @@ def _state8_call(state: AdamState8, exp_avgs, exp_avg_sqs, write: int) -> None:
     words = _words(n, _ptrs(exp_avgs), _ptrs(exp_avg_sqs), _ptrs(state.exp_avg), _ptrs(state.root), _ptrs(state.exp_avg_scale), _ptrs(state.root_scale),
                    numel, None, [(L.F32 << 32) | (8 << 48)] * n)
     _run(device, "nndet_adam_state8", words, n, write)
+    _written(out)
 
 
 def write_adam_state8(state: AdamState8, exp_avgs, exp_avg_sqs) -> None:

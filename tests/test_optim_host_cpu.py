@@ -196,3 +196,17 @@ def test_tensors_with_a_negation_to_come(monkeypatch):
     with pytest.raises(L.NndetError, match="grad_scale"):
         O.adamw_step([p], [g], [m], [v], steps, lr=0.1, grad_scale=mk(-2.0)[0])
     assert len(seen) == 3
+
+
+def test_written_states_have_another_version(monkeypatch):
+    monkeypatch.setattr(O, "_run", lambda *args: None)
+    m, v = [torch.zeros(300)], [torch.zeros(300)]
+    st = O.AdamState8.zeros(m)
+    codes = [t for ts in st for t in ts]
+    count = lambda ts: [t._version for t in ts]  # noqa: E731
+    a, b = count(codes), count(m + v)
+    O.write_adam_state8(st, m, v)
+    assert all(x > y for x, y in zip(count(codes), a)) and count(m + v) == b
+    a = count(codes)
+    O.read_adam_state8(st, m, v)
+    assert all(x > y for x, y in zip(count(m + v), b)) and count(codes) == a
