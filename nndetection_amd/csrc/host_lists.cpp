@@ -70,6 +70,12 @@ struct Addresses {                                   // a set of addresses: open
             if (!slot[i]) { slot[i] = p; return true; }
         }
     }
+    bool has(const void* p) const {
+        for (size_t i = ((uintptr_t)p >> 4) * 0x9E3779B97F4A7C15ull >> 32 & mask;; i = (i + 1) & mask) {
+            if (slot[i] == p) return true;
+            if (!slot[i]) return false;
+        }
+    }
 };
 
 // pack(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, root_scales, weight_decay, bits, device, both)
@@ -96,7 +102,7 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         PyObject* out = PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(NndetOptTensor));
         if (!out) return nullptr;
         NndetOptTensor* t = reinterpret_cast<NndetOptTensor*>(PyBytes_AS_STRING(out));
-        Addresses seen((p.seq ? 1 + (both != 0) : 1) * n + (m.seq ? 2 * n : 0));
+        Addresses seen((p.seq ? 1 + (both != 0) : 1) * n + (m.seq ? 2 * n : 0) + (ms.seq ? 2 * n : 0));
         Py_ssize_t k = 0;
         for (Py_ssize_t i = 0; i < n; ++i) {
             c10::TensorImpl *px = nullptr, *gx = nullptr;
@@ -149,9 +155,13 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             if (e.numel) {                           // what a call writes: no address twice
                 if (!seen.add(px ? e.param : e.grad) || (px && both && !seen.add(e.grad))) goto other;
                 if (m.seq && (!seen.add(e.exp_avg) || !seen.add(e.exp_avg_sq))) goto other;
+                if (e.state_bits == 8 && (!seen.add(e.exp_avg_scale) || !seen.add(e.root_scale))) goto other;
             }
             ++k;
         }
+        if (p.seq && !both)                          // what it reads: a gradient may be its own tensor's memory, but no other's
+            for (Py_ssize_t i = 0; i < k; ++i)
+                if (t[i].numel && seen.has(t[i].grad) && t[i].grad != t[i].param && t[i].grad != t[i].exp_avg && t[i].grad != t[i].exp_avg_sq) goto other;
         if (k != n && _PyBytes_Resize(&out, k * (Py_ssize_t)sizeof(NndetOptTensor)) < 0) return nullptr;
         return Py_BuildValue("Nn", out, k);
     other:

@@ -221,6 +221,14 @@ def _check_distinct(name: str, ts) -> None:
         _refuse(f"the same tensor twice in {name}: its updates would race")
 
 
+def _check_read(grads, *written) -> None:
+    """No gradient is memory that the call writes for ANOTHER tensor (its own is read before it is written)."""
+    at = {t.data_ptr(): i for ts in written for i, t in enumerate(ts) if t.numel()}
+    for i, g in enumerate(grads):
+        if at.get(g.data_ptr(), i) != i:
+            _refuse(f"the gradient of tensor {i} is memory that the call writes for tensor {at[g.data_ptr()]}")
+
+
 def _scalar(name: str, t, device) -> Optional[int]:
     """Address of a one-element fp32 tensor on `device`, None for None."""
     if t is None:
@@ -358,7 +366,8 @@ def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight
     if bits == 8:
         for name, ts in (("exp_avg_scale", ms), ("root_scale", rs)):
             _check_scales(name, ts, numel, device)
-    _check_distinct("params and moments", [*params, *m, *v])
+    _check_distinct("params and moments", [*params, *m, *v, *(ms or ()), *(rs or ())])
+    _check_read(grads, params, m, v)
     bits_of = {w: _double_bits(float(w)) for w in set(wd)}
     words = _words(n, _ptrs(params), _ptrs(grads), _ptrs(m), _ptrs(v), ms and _ptrs(ms), rs and _ptrs(rs), numel, [bits_of[w] for w in wd],
                    [s | k | (bits << 48) for s, k in zip(slots, kinds)])
@@ -481,7 +490,7 @@ def _state8_call(state: AdamState8, exp_avgs, exp_avg_sqs, write: int) -> None:
     numel = [t.numel() for t in exp_avgs]
     _check_scales("exp_avg_scale", state.exp_avg_scale, numel, device)
     _check_scales("root_scale", state.root_scale, numel, device)
-    _check_distinct("what is written", [*state.exp_avg, *state.root] if write else [*exp_avgs, *exp_avg_sqs])
+    _check_distinct("what is written", out)
     words = _words(n, _ptrs(exp_avgs), _ptrs(exp_avg_sqs), _ptrs(state.exp_avg), _ptrs(state.root), _ptrs(state.exp_avg_scale), _ptrs(state.root_scale),
                    numel, None, [(L.F32 << 32) | (8 << 48)] * n)
     _run(device, "nndet_adam_state8", words, n, write)
@@ -630,7 +639,9 @@ class AdamW:
                 per.setdefault(device, []).extend(c[2])
             norms = [grad_norm(gs, on(scale, device)) for device, gs in per.items()]
             total = norms[0] if len(norms) == 1 else torch.stack([x.to(norms[0].device, torch.float64) for x in norms]).square().sum().sqrt().float()
-        _check_distinct("the parameters", [p for c in calls.values() for p in c[1]])
+        ps, gs = ([t for c in calls.values() for t in c[i]] for i in (1, 2))
+        _check_distinct("the parameters", ps)
+        _check_read(gs, ps)
         for (device, _), (words, ps, _, g) in calls.items():
             counts = self._counts(device)
             a, self.grad_norm = _hyper(g["lr"], g["betas"], g["eps"], self.max_norm, on(total, device), on(scale, device), on(found, device),

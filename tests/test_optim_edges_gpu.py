@@ -283,3 +283,14 @@ def test_an_optimizer_of_both_kinds_of_moments_with_many_tensors(clip):
             assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
     kinds = [("root" in st) for st in opt.state_dict()["state"].values()]
     assert sum(kinds) == 90 and len(kinds) == 210
+
+
+def test_memory_that_is_written_for_another_tensor_is_refused():
+    """Through the fast path too, before anything runs."""
+    from tests.test_optim_host_cpu import overlapping
+    for match, call in overlapping(DEV):
+        if match:
+            with pytest.raises(L.NndetError, match=match):
+                call()
+        else:
+            call()

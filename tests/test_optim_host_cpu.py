@@ -210,3 +210,33 @@ def test_written_states_have_another_version(monkeypatch):
     a = count(codes)
     O.read_adam_state8(st, m, v)
     assert all(x > y for x, y in zip(count(m + v), b)) and count(codes) == a
+
+
+def overlapping(dev):
+    """Calls in which one tensor's memory is written for another, and two that are fine: (refused or not, call)."""
+    mk = lambda n=300: torch.zeros(n, device=dev)  # noqa: E731
+    p, g, m, v, steps = [mk(), mk()], [mk(), mk()], [mk(), mk()], [mk(), mk()], torch.zeros(2, dtype=torch.int32, device=dev)
+    st = O.AdamState8.zeros(p)
+    one = torch.zeros(2, device=dev)
+    params = [torch.nn.Parameter(t) for t in p]
+    opt = O.AdamW([{"params": params[:1], "lr": 0.1}, {"params": params[1:], "lr": 0.2}])
+    params[0].grad, params[1].grad = g[0], p[0]
+    return [("tensor 1 is memory", lambda: O.adamw_step(p, [g[0], p[0]], m, v, steps, lr=0.1)), ("tensor 0 is memory", lambda: O.adamw_step(p, [v[1], g[1]], m, v, steps, lr=0.1)),
+            ("twice", lambda: O.adamw8_step(p, g, st._replace(root_scale=st.exp_avg_scale), steps, lr=0.1)),
+            ("twice", lambda: O.adamw8_step(p, g, st._replace(root_scale=[one, one]), steps, lr=0.1)),
+            ("twice", lambda: O.write_adam_state8(st._replace(exp_avg_scale=[one, one]), m, v)), ("tensor 1 is memory", opt.step),
+            (None, lambda: O.adamw_step(p, [g[0], g[0]], m, v, steps, lr=0.1)), (None, lambda: O.adamw_step(p, p, m, v, steps, lr=0.1)),
+            (None, lambda: O.read_adam_state8(st._replace(exp_avg_scale=[one, one]), m, v))]
+
+
+def test_memory_that_is_written_for_another_tensor_is_refused(monkeypatch):
+    ran = []
+    monkeypatch.setattr(O, "_run", lambda *args: ran.append(args[1]))
+    monkeypatch.setattr(O.AdamW, "_init_state", lambda self, p: self._set_state(p, {"exp_avg": torch.zeros(300), "exp_avg_sq": torch.zeros(300)}))
+    for match, call in overlapping("cpu"):
+        if match:
+            with pytest.raises(L.NndetError, match=match):
+                call()
+        else:
+            call()
+    assert len(ran) == 3
