@@ -409,7 +409,9 @@ def adamw8_step(params, grads, state: AdamState8, steps: torch.Tensor, *, lr: Ra
                 found_inf: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """`adamw_step` with the moments in 8 bits: 2.03 bytes an element instead of 8. The step itself is computed in fp32 from the moments as
     they are stored; the new ones are then rounded, the first to the nearest code, the root of the second up or down with the probability
-    that keeps its expected value (by bits that follow from the element's index and its step count: the same step gives the same state).
+    that keeps the root's expected value (by bits that follow from the element's index and its step count: the same step gives the same state).
+    The expected value of its square is then larger by the variance of the rounding, and the recursion adds that up: with gradients of a fixed
+    normal distribution the second moment settles 5 - 6 % too large (2 - 5 % for b2 <= 0.99), its root 1.3 %; state_dict(bits=32) and `read_adam_state8` pass it on.
     A gradient that is not finite makes the moments of its whole block NaN; `found_inf` keeps it out."""
     m, ms, v, rs = state
     return _adamw_call(params, grads, m, v, ms, rs, 8, steps, lr, betas, eps, weight_decay, max_norm, total_norm, grad_scale, found_inf)

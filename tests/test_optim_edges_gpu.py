@@ -7,7 +7,7 @@ import torch
 
 from nndetection_amd import _lib as L
 from nndetection_amd import optim as O
-from tests.test_optim_gpu import DEV, U, check8, formula, gen, guards_intact, make, rows, within, test_norm_and_clip as norm_and_clip
+from tests.test_optim_gpu import BLOCK, DEV, U, check8, formula, gen, guards_intact, make, rows, within, test_norm_and_clip as norm_and_clip
 
 pytestmark = pytest.mark.gpu
 TINY = 2.0 ** -149                                   # one denormal step
@@ -294,3 +294,45 @@ def test_memory_that_is_written_for_another_tensor_is_refused():
                 call()
         else:
             call()
+
+
+def test_the_second_moment_of_many_8_bit_steps():
+    """600 steps at b2 = 0.99 with gradients drawn from four magnitudes: the mean second moment is that of the format's own recursion -- a Markov chain
+    over the 127 codes, exact in 64 bits -- and that lies 0 .. 8 % above the mean square of the gradients, which is what 32-bit moments settle at.
+
+    One element of each block has the gradient that keeps it at 448, so every scale stays 1. The mean over n independent elements is off by at most
+    6 standard deviations / sqrt(n). The kernel's probabilities are multiples of 2^-16 taken at their middle: a step is off by 2^-17 of a code's distance (at
+    most r / 8, i.e. 2^-19 of v), and 1 / (1 - b2) steps add up: 100 * 2^-19 of v."""
+    n, b2, N = 256 * 256, 0.99, 600
+    sizes = [4.0, 12.0, 20.0, 40.0]
+    code = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    T = torch.zeros(127, 127, dtype=torch.float64)
+    for a in sizes:
+        r = (b2 * code * code + (1 - b2) * a * a).sqrt()
+        lo = (torch.searchsorted(code, r, right=True) - 1).clamp(0, 125)
+        up = ((r - code[lo]) / (code[lo + 1] - code[lo])).clamp(0, 1)
+        assert int(lo.min()) > 0                     # (never near the least code, which has a rule of its own)
+        T[torch.arange(127), lo] += (1 - up) / 4
+        T[torch.arange(127), lo + 1] += up / 4
+    at = torch.zeros(127, dtype=torch.float64)
+    at[(code == 24.0).nonzero()] = 1.0               # the start: r = 24, a code
+    for _ in range(N):
+        at = at @ T
+    mean = float(at @ code ** 2)
+    var = float(at @ code ** 4) - mean ** 2
+    true = sum(a * a for a in sizes) / 4
+    assert 1.0 < mean / true < 1.08
+    r = torch.full((n,), 24.0, device=DEV)
+    r[::BLOCK] = 448.0
+    p, st, steps = torch.zeros(n, device=DEV), O.AdamState8.zeros([r]), torch.zeros(1, dtype=torch.int32, device=DEV)
+    O.write_adam_state8(st, [torch.zeros(n, device=DEV)], [r * r])
+    table, g = torch.tensor(sizes, device=DEV), gen(12)
+    for _ in range(N):
+        grad = table[torch.randint(0, 4, (n,), generator=g, device=DEV)]
+        grad[::BLOCK] = 448.0
+        O.adamw8_step([p], [grad], st, steps, lr=0.0, betas=(0.9, b2))
+    assert bool((st.root_scale[0] - 1).abs().max() <= N * 4 * U)
+    got = rows(st.root[0].float()).double()[:, 1:].square().mean()
+    count = 255 * 256
+    assert abs(float(got) - mean) <= 6 * math.sqrt(var / count) + 100 * 2.0 ** -19 * mean + N * 16 * U * mean
+    assert float(got) > true                         # (the bias that the documentation states is there)
