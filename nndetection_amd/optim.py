@@ -12,6 +12,7 @@ AdamW and clipping: HIP kernels over all tensors of a call at once (csrc/optim.h
 current stream of the tensors' device, never wait for the GPU, and can be captured into a HIP graph.
 """
 import array
+import operator
 import os
 import struct
 from typing import List, NamedTuple, Optional, Sequence, Union
@@ -596,7 +597,9 @@ class AdamW:
         if len(keys) == 1 and len(self._steps) == 1:         # one call; None if a state is missing or anything is out of the ordinary
             (device, counts), = self._steps.items()
             wds = [g["weight_decay"] for g in self.param_groups for _ in g["params"]]
-            packed = _pack(device, self._flat, None, *self._lists, wds, 0)
+            # (a parameter may have been moved to another group, or left out, since the lists were made)
+            as_made = len(wds) == len(self._flat) and all(map(operator.is_, (p for g in self.param_groups for p in g["params"]), self._flat))
+            packed = _pack(device, self._flat, None, *self._lists, wds, 0) if as_made else None
             if packed is not None:
                 if packed[1]:
                     g = self.param_groups[0]

@@ -336,3 +336,23 @@ def test_the_second_moment_of_many_8_bit_steps():
     count = 255 * 256
     assert abs(float(got) - mean) <= 6 * math.sqrt(var / count) + 100 * 2.0 ** -19 * mean + N * 16 * U * mean
     assert float(got) > true                         # (the bias that the documentation states is there)
+
+
+def test_parameters_that_change_their_group():
+    """The groups are read at every step: a parameter takes the decay of the group it is in, one that was taken out stays as it is."""
+    ps = [torch.nn.Parameter(torch.randn(300, generator=gen(i), device=DEV)) for i in range(3)]
+    opt = O.AdamW([{"params": ps[:2], "weight_decay": 0.5}, {"params": ps[2:], "weight_decay": 0.0}], lr=0.1)
+    random_grads(ps, 20)
+    opt.step()
+    a, b = (g["params"] for g in opt.param_groups)
+    for change, decays in ((lambda: (b.insert(0, a.pop(1))), (0.5, 0.0, 0.0)), (lambda: (a.append(b.pop(1)), b.append(a.pop(0))), (0.0, 0.0, 0.5)), (lambda: a.pop(0), (0.0, 0.0, None))):
+        change()
+        old = [p.detach().clone() for p in ps]
+        st = {i: {k: v.clone() for k, v in opt._state[p].items()} for i, p in enumerate(ps)}
+        t = [int(opt._steps[ps[0].device][i]) + 1 for i in range(3)]
+        opt.step()
+        for i, (p, wd) in enumerate(zip(ps, decays)):
+            if wd is None:
+                assert torch.equal(p, old[i])
+            else:
+                within(p.detach(), *formula(old[i], p.grad, st[i]["exp_avg"], st[i]["exp_avg_sq"], t[i], 0.1, 0.9, 0.999, 1e-8, wd)[0], what=f"{i}")
