@@ -598,7 +598,7 @@ class AdamW:
             (device, counts), = self._steps.items()
             wds = [g["weight_decay"] for g in self.param_groups for _ in g["params"]]
             # (a parameter may have been moved to another group, or left out, since the lists were made)
-            as_made = len(wds) == len(self._flat) and all(map(operator.is_, (p for g in self.param_groups for p in g["params"]), self._flat))
+            as_made = len(wds) == len(self._flat) and all(map(operator.is_, self._in_order(), self._flat))
             packed = _pack(device, self._flat, None, *self._lists, wds, 0) if as_made else None
             if packed is not None:
                 if packed[1]:
@@ -677,9 +677,13 @@ class AdamW:
                            "differentiable": False, "fused": None, "decoupled_weight_decay": True, "params": ids})
         return {"state": state, "param_groups": groups}
 
+    def _in_order(self) -> list:
+        """The parameters of the groups as they are now: what the numbers in a checkpoint count."""
+        return [p for g in self.param_groups for p in g["params"]]
+
     def _check_loaded(self, sd: dict) -> None:
         """Everything that load_state_dict wants of a checkpoint, before it touches the optimiser."""
-        groups = sd["param_groups"]
+        groups, flat = sd["param_groups"], self._in_order()
         if len(groups) != len(self.param_groups) or any(len(a["params"]) != len(b["params"]) for a, b in zip(groups, self.param_groups)):
             raise ValueError("loaded state dict has different parameter groups")
         if any(g.get("amsgrad") or g.get("maximize") for g in groups):
@@ -691,9 +695,9 @@ class AdamW:
             float(g["lr"])
             _check_group(float(g["weight_decay"]), g["betas"], float(g["eps"]))
         for k, st in sd["state"].items():
-            if not 0 <= int(k) < len(self._flat):
-                raise ValueError(f"loaded state of parameter {k}: there are {len(self._flat)}")
-            p = self._flat[int(k)]
+            if not 0 <= int(k) < len(flat):
+                raise ValueError(f"loaded state of parameter {k}: there are {len(flat)}")
+            p = flat[int(k)]
             names = AdamState8._fields if "root" in st else ("exp_avg", "exp_avg_sq")
             missing = [c for c in ("step", *names) if c not in st]
             if missing:
@@ -711,10 +715,11 @@ class AdamW:
     def load_state_dict(self, sd: dict) -> None:
         """A checkpoint that does not fit is refused and changes nothing. The state is made anew: a captured step has to be captured again."""
         self._check_loaded(sd)
+        flat = self._in_order()
         like = lambda t, p, dtype: torch.empty_like(p, dtype=dtype).copy_(t.detach())  # noqa: E731
         state, counts = {}, {}
         for k, st in sd["state"].items():
-            p = self._flat[int(k)]
+            p = flat[int(k)]
             if "root" in st:                         # in their own memory order: a scale belongs to consecutive elements
                 at = lambda t: t.detach().to(p.device, copy=True)  # noqa: E731
                 st8 = AdamState8([at(st["exp_avg"].view(torch.uint8)).view(_F8)], [at(st["exp_avg_scale"]).contiguous()],

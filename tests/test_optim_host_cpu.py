@@ -240,3 +240,19 @@ def test_memory_that_is_written_for_another_tensor_is_refused(monkeypatch):
         else:
             call()
     assert len(ran) == 3
+
+
+def test_checkpoints_follow_the_groups_as_they_are():
+    """Numbers in a checkpoint run over the groups in order, also after a parameter was moved to another one."""
+    ps = [torch.nn.Parameter(torch.zeros(k)) for k in (3, 4, 5)]
+    opt = stepped([*ps])
+    opt.param_groups.append(dict(opt.param_groups[0], params=[opt.param_groups[0]["params"].pop(0)], weight_decay=0.0))
+    sd = copy.deepcopy(opt.state_dict())
+    assert [tuple(sd["state"][i]["exp_avg"].shape) for i in range(3)] == [(4,), (5,), (3,)]
+    sd["state"][2]["step"] = 9
+    opt.load_state_dict(sd)
+    assert [float(opt._state[p]["exp_avg"][0]) for p in ps] == [1.0, 2.0, 3.0] and opt._counts(ps[0].device).tolist() == [9, 5, 5]
+    opt.param_groups.pop()                           # a parameter that is left out has no number
+    assert sorted(opt.state_dict()["state"]) == [0, 1]
+    with pytest.raises(ValueError, match="different parameter groups"):
+        opt.load_state_dict(sd)
