@@ -33,7 +33,7 @@ c10::TensorImpl* plain(const at::TensorBase& t, c10::DeviceIndex device) {
     c10::TensorImpl* x = t.unsafeGetTensorImpl();
     if (x->layout() != c10::kStrided || x->is_python_dispatch() || x->device() != c10::Device(c10::kCUDA, device)) return nullptr;
     if (x->key_set().has(c10::DispatchKey::Negative)) return nullptr;     // (the sign is still to be changed)
-    if (!(x->is_contiguous() || x->is_non_overlapping_and_dense()) || (x->numel() && !x->data())) return nullptr;
+    if (!(x->is_contiguous() || x->is_non_overlapping_and_dense())) return nullptr;
     return x;
 }
 c10::TensorImpl* plain(PyObject* o, c10::DeviceIndex device) {

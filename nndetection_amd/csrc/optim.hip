@@ -975,7 +975,6 @@ extern "C" int nndet_adam_state8(const NndetOptTensor* tensors, int32_t n, int32
     const int k = NNDET_F32 + 3;
     if (!P.tiles[k]) return 0;
     const unsigned g = opt_grid(P.tiles[k], OPT_GRID);
-    const int m = P.first[k + 1] - P.first[k];
     if (write) k_opt_state8<true><<<g, OPT_WG, 0, st>>>(opt_mem(P, k), (uint32_t)P.tiles[k]);
     else k_opt_state8<false><<<g, OPT_WG, 0, st>>>(opt_mem(P, k), (uint32_t)P.tiles[k]);
     LAUNCH_CHECK();

@@ -12,6 +12,7 @@ AdamW and clipping: HIP kernels over all tensors of a call at once (csrc/optim.h
 current stream of the tensors' device, never wait for the GPU, and can be captured into a HIP graph.
 """
 import array
+import ctypes as C
 import operator
 import os
 import struct
@@ -278,9 +279,11 @@ def _ptrs(ts) -> list:
     return [t.data_ptr() for t in ts]
 
 
-def _written(ts) -> None:
+def _written(*lists) -> None:
     """The kernels write through raw pointers: advance the version counters as torch's in-place operators do."""
-    L.host_lists().written(list(ts), None)
+    written = L.host_lists().written
+    for ts in lists:
+        written(ts, None)
 
 
 def _pack(device, params, grads, m, v, ms, rs, wd, bits: int, both: bool = False):
@@ -345,7 +348,7 @@ def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight
     a, norm = _hyper(lr, betas, eps, max_norm, total_norm, grad_scale, found_inf, steps, steps.device)
     packed = _pack(steps.device, params, grads, m, v, ms, rs, weight_decay, bits)
     if packed is not None:
-        if _run(steps.device, "nndet_adamw_step", *packed, L.C.byref(a)):
+        if _run(steps.device, "nndet_adamw_step", *packed, C.byref(a)):
             L.note_graph_write([p for p, g in zip(params, grads) if g is not None])
         L.host_lists().written(params, grads)
         return norm
@@ -372,7 +375,7 @@ def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight
     bits_of = {w: _double_bits(float(w)) for w in set(wd)}
     words = _words(n, _ptrs(params), _ptrs(grads), _ptrs(m), _ptrs(v), ms and _ptrs(ms), rs and _ptrs(rs), numel, [bits_of[w] for w in wd],
                    [s | k | (bits << 48) for s, k in zip(slots, kinds)])
-    if _run(device, "nndet_adamw_step", words, n, L.C.byref(a)):
+    if _run(device, "nndet_adamw_step", words, n, C.byref(a)):
         L.note_graph_write(params)
     _written(params)
     return norm
@@ -481,11 +484,11 @@ def _state8_call(state: AdamState8, exp_avgs, exp_avg_sqs, write: int) -> None:
     if n == 0:
         return
     device = exp_avgs[0].device
-    out = [t for ts in state for t in ts] if write else [*exp_avgs, *exp_avg_sqs]
+    out = state if write else (exp_avgs, exp_avg_sqs)
     packed = _pack(device, exp_avgs, exp_avg_sqs, state.exp_avg, state.root, state.exp_avg_scale, state.root_scale, 0.0, 8, True)
     if packed is not None and exp_avgs[0].dtype == torch.float32:
         _run(device, "nndet_adam_state8", *packed, write)
-        return _written(out)
+        return _written(*out)
     _check_list("exp_avgs", exp_avgs, torch.float32, device)
     _check_list("exp_avg_sqs", exp_avg_sqs, torch.float32, device, exp_avgs)
     _check_list("exp_avg", state.exp_avg, _F8, device, exp_avgs)
@@ -493,11 +496,11 @@ def _state8_call(state: AdamState8, exp_avgs, exp_avg_sqs, write: int) -> None:
     numel = [t.numel() for t in exp_avgs]
     _check_scales("exp_avg_scale", state.exp_avg_scale, numel, device)
     _check_scales("root_scale", state.root_scale, numel, device)
-    _check_distinct("what is written", out)
+    _check_distinct("what is written", [t for ts in out for t in ts])
     words = _words(n, _ptrs(exp_avgs), _ptrs(exp_avg_sqs), _ptrs(state.exp_avg), _ptrs(state.root), _ptrs(state.exp_avg_scale), _ptrs(state.root_scale),
                    numel, None, [(L.F32 << 32) | (8 << 48)] * n)
     _run(device, "nndet_adam_state8", words, n, write)
-    _written(out)
+    _written(*out)
 
 
 def write_adam_state8(state: AdamState8, exp_avgs, exp_avg_sqs) -> None:
@@ -589,31 +592,57 @@ class AdamW:
         for ts, k in zip(self._lists, ("exp_avg", "root" if "root" in st else "exp_avg_sq", "exp_avg_scale", "root_scale")):
             ts[self._slot[p]] = st.get(k)
 
+    @staticmethod
+    def _key(g) -> tuple:
+        """What the parameters of one call share."""
+        return (id(g["lr"]) if isinstance(g["lr"], torch.Tensor) else g["lr"], *g["betas"], g["eps"])
+
+    def _packed_step(self, device, counts, words, n: int, scale, found) -> None:
+        """The step of the `n` tensors in `words` (those of self._flat with a gradient, in order): one call, or one for each key."""
+        on = lambda t: None if t is None else t.to(device)  # noqa: E731
+        scale, found, total = on(scale), on(found), None
+        ps = self._flat if n == len(self._flat) else [p for p in self._flat if p.grad is not None]
+        calls = {self._key(g): (g, []) for g in self.param_groups}
+        if len(calls) == 1:
+            calls = [(g, words, n, ps) for g, _ in calls.values()]
+        else:
+            i = 0
+            for g in self.param_groups:
+                of_key = calls[self._key(g)][1]
+                for p in g["params"]:
+                    if p.grad is not None:
+                        of_key.append(i)
+                        i += 1
+            size = C.sizeof(L.NndetOptTensor)
+            calls = [(g, b"".join([words[size * i:size * (i + 1)] for i in own]), len(own), [ps[i] for i in own]) for g, own in calls.values() if own]
+            if self.max_norm is not None and len(calls) > 1:     # a norm over all of them first
+                total = grad_norm([p.grad for p in ps], scale)
+        for g, words, n, ps in calls:
+            a, self.grad_norm = _hyper(g["lr"], g["betas"], g["eps"], self.max_norm, total, scale, found, counts, device)
+            if _run(device, "nndet_adamw_step", words, n, C.byref(a)):
+                L.note_graph_write(ps)
+            _written(ps)
+
     @torch.no_grad()
     def step(self) -> None:
         scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
         self.grad_norm = None
-        keys = {(id(g["lr"]) if isinstance(g["lr"], torch.Tensor) else g["lr"], *g["betas"], g["eps"]) for g in self.param_groups}
-        if len(keys) == 1 and len(self._steps) == 1:         # one call; None if a state is missing or anything is out of the ordinary
+        if len(self._steps) == 1:                    # the ordinary case; None if a state is missing or anything is out of the ordinary
             (device, counts), = self._steps.items()
-            wds = [g["weight_decay"] for g in self.param_groups for _ in g["params"]]
+            flat, wds = self._in_order(), []
+            for g in self.param_groups:
+                wds += [g["weight_decay"]] * len(g["params"])
             # (a parameter may have been moved to another group, or left out, since the lists were made)
-            as_made = len(wds) == len(self._flat) and all(map(operator.is_, self._in_order(), self._flat))
-            packed = _pack(device, self._flat, None, *self._lists, wds, 0) if as_made else None
+            as_made = len(flat) == len(self._flat) and all(map(operator.is_, flat, self._flat))
+            packed = _pack(device, flat, None, *self._lists, wds, 0) if as_made else None
             if packed is not None:
                 if packed[1]:
-                    g = self.param_groups[0]
-                    on = lambda t: None if t is None else t.to(device)  # noqa: E731
-                    a, self.grad_norm = _hyper(g["lr"], g["betas"], g["eps"], self.max_norm, None, on(scale), on(found), counts, device)
-                    ps = self._flat if packed[1] == len(self._flat) else [p for p in self._flat if p.grad is not None]
-                    if _run(device, "nndet_adamw_step", *packed, L.C.byref(a)):
-                        L.note_graph_write(ps)
-                    _written(ps)
+                    self._packed_step(device, counts, *packed, scale, found)
                 return
         calls = {}
         for g in self.param_groups:
             wd = _double_bits(float(g["weight_decay"]))
-            key = (id(g["lr"]) if isinstance(g["lr"], torch.Tensor) else g["lr"], *g["betas"], g["eps"])
+            key = self._key(g)
             for p in g["params"]:
                 gr = p.grad
                 if gr is None:
@@ -651,7 +680,7 @@ class AdamW:
             counts = self._counts(device)
             a, self.grad_norm = _hyper(g["lr"], g["betas"], g["eps"], self.max_norm, on(total, device), on(scale, device), on(found, device),
                                        counts, device)
-            if _run(device, "nndet_adamw_step", array.array("q", words).tobytes(), len(ps), L.C.byref(a)):
+            if _run(device, "nndet_adamw_step", array.array("q", words).tobytes(), len(ps), C.byref(a)):
                 L.note_graph_write(ps)
             _written(ps)
 
@@ -679,7 +708,10 @@ class AdamW:
 
     def _in_order(self) -> list:
         """The parameters of the groups as they are now: what the numbers in a checkpoint count."""
-        return [p for g in self.param_groups for p in g["params"]]
+        ps = []
+        for g in self.param_groups:
+            ps += g["params"]
+        return ps
 
     def _check_loaded(self, sd: dict) -> None:
         """Everything that load_state_dict wants of a checkpoint, before it touches the optimiser."""

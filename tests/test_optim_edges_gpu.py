@@ -356,3 +356,36 @@ def test_parameters_that_change_their_group():
                 assert torch.equal(p, old[i])
             else:
                 within(p.detach(), *formula(old[i], p.grad, st[i]["exp_avg"], st[i]["exp_avg_sq"], t[i], 0.1, 0.9, 0.999, 1e-8, wd)[0], what=f"{i}")
+
+
+@pytest.mark.parametrize("clip", [False, True])
+def test_three_rates_after_the_first_step(clip):
+    """Parameters of one rate scattered over the groups, some without a gradient, a rate whose parameters have none: one call a rate, one norm over all."""
+    ps = [torch.nn.Parameter(torch.randn(k, generator=gen(k), device=DEV)) for k in (300, 5, 4097, 64, 1000, 7)]
+    lr = torch.tensor(0.05, device=DEV)
+    groups = [dict(params=[ps[0], ps[1]], lr=0.1, weight_decay=0.1), dict(params=[ps[2]], lr=lr, weight_decay=0.2), dict(params=[ps[3], ps[4]], lr=0.1, weight_decay=0.0),
+              dict(params=[ps[5]], lr=0.3, weight_decay=0.3)]
+    rates = [0.1, 0.1, float(lr), 0.1, 0.1, 0.3]
+    decays = [0.1, 0.1, 0.2, 0.0, 0.0, 0.3]
+    opt = O.AdamW(groups, max_norm=0.5 if clip else None)
+    random_grads(ps, 30)
+    opt.step()
+    for without in ((), (1,), (5,), (0, 1, 3, 4, 5)):
+        random_grads(ps, 40 + len(without))
+        for i in without:
+            ps[i].grad = None
+        live = [i for i in range(6) if i not in without]
+        norm = math.sqrt(sum(float(ps[i].grad.double().square().sum()) for i in live))
+        factor = min(1.0, 0.5 / (norm + 1e-6)) if clip else 1.0
+        st = {i: {k: v.clone() for k, v in opt._state[p].items()} for i, p in enumerate(ps)}
+        t = opt._steps[ps[0].device].tolist()
+        old = [p.detach().clone() for p in ps]
+        opt.step()
+        for i, p in enumerate(ps):
+            if i in without:
+                assert torch.equal(p, old[i])
+                continue
+            wp, _, _ = formula(old[i], p.grad, st[i]["exp_avg"], st[i]["exp_avg_sq"], t[i] + 1, rates[i], 0.9, 0.999, 1e-8, decays[i], factor)
+            within(p.detach(), wp[0], 1.5 * wp[1], what=str(i))
+        assert opt._steps[ps[0].device].tolist() == [k + (i not in without) for i, k in enumerate(t)]
+        assert opt.grad_norm is None if not clip else abs(float(opt.grad_norm) - norm) <= 2 * U * norm
