@@ -220,7 +220,8 @@ template <int NB, typename S> struct OptWalk {
 template <typename T> using OptPtr = __attribute__((address_space(1))) T*;
 template <typename T> __device__ __forceinline__ OptPtr<T> opt_at(const void* p, int64_t i) { return (OptPtr<T>)(uintptr_t)p + i; }
 // STREAM: nontemporal. What a step reads and writes once would only push the rest out of the caches: with plain accesses the step of 295 M
-// parameters takes 1.54 ms instead of 1.40 (nontemporal loads or stores alone: 1.57 - 1.60), reading the 8-bit moments 0.58 instead of 0.53 ms.
+// parameters takes 1.57 ms instead of 1.46 (nontemporal loads alone 1.585, stores alone 1.57), a clipped one with 8-bit moments 1.11 instead of 0.96, reading
+// the 8-bit moments 0.514 instead of 0.503 (stores alone: 0.491).
 template <typename T> struct OptVec4;
 template <> struct OptVec4<float> { typedef f32x4 type; };
 template <> struct OptVec4<bf16_t> { typedef bf16_t type __attribute__((ext_vector_type(4))); };
@@ -286,8 +287,9 @@ __device__ __forceinline__ void opt_decode(uint32_t c, float s, float* x) {
     x[0] = lo[0] * s; x[1] = lo[1] * s; x[2] = hi[0] * s; x[3] = hi[1] * s;
 }
 // Square root and quotient of the 8-bit step, which with the IEEE sequences kept its vector units busy for 73 % (19.0 M elements) to 94 % (295 M) of
-// the time: 85 instructions an element, now 65. 19 and 13 issue slots for those sequences, 11 and 8 for these: 60.5 -> 57.7 us at 19.0 M, no change at
-// 295 M; with 16-bit parameters (10 B an element) the vector units stay the bound: 60 M elements of fp16 146 -> 136 us (4.4 TB/s), of bf16 128 -> 124.
+// the time with 85 instructions an element; now 64, 57 % and 77 %. 19 and 13 issue slots for those sequences, 12 and 8 for these: 60.5 -> 57.7 us at
+// 19.0 M, no change at 295 M. With 16-bit parameters (10 B an element) the vector units are the bound of large calls: 66 (fp16) and 72 (bf16) instructions an
+// element, busy all the time at 60 M elements (122 and 121 us, 5.0 TB/s); at 6.2 M (17 us) 43 % of it, in 1.7 rounds of workgroups.
 // One residual step behind the hardware's reciprocal (root): correctly rounded but for about one value in 2^22.
 __device__ __forceinline__ float opt_root(float v) {
     const float y = __builtin_amdgcn_rsqf(v), s = v * y;
