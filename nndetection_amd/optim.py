@@ -333,8 +333,8 @@ def _hyper(lr, betas, eps, max_norm, total_norm, grad_scale, found_inf, steps, d
 
 
 def _listed(*args):
-    """Each argument as a list or tuple (None stays None)."""
-    return [x if x is None or isinstance(x, (list, tuple)) else list(x) for x in args]
+    """Each argument as a list or tuple (None stays None); a class derived from list becomes one."""
+    return [x if x is None or type(x) is list or isinstance(x, tuple) else list(x) for x in args]
 
 
 def _adamw_call(params, grads, m, v, ms, rs, bits, steps, lr, betas, eps, weight_decay, max_norm, total_norm, grad_scale, found_inf):

@@ -256,3 +256,19 @@ def test_checkpoints_follow_the_groups_as_they_are():
     assert sorted(opt.state_dict()["state"]) == [0, 1]
     with pytest.raises(ValueError, match="different parameter groups"):
         opt.load_state_dict(sd)
+
+
+def test_lists_of_a_derived_class(monkeypatch):
+    ran = []
+    monkeypatch.setattr(O, "_run", lambda *args: ran.append(args[1]))
+
+    class Mine(list):
+        pass
+
+    p, g, m, v = (Mine([torch.zeros(3)]) for _ in range(4))
+    O.adamw_step(p, g, m, v, torch.zeros(1, dtype=torch.int32), lr=0.1)
+    O.clip_grads_(g, 1.0)
+    st = O.AdamState8(*(Mine(x) for x in O.AdamState8.zeros(m)))
+    O.write_adam_state8(st, m, v)
+    O.read_adam_state8(st, m, v)
+    assert len(ran) == 4
