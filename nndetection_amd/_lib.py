@@ -476,9 +476,9 @@ def graph_task_id() -> int:
 
 # Parameters that a captured optimiser step writes (AdamW): their version counters advance when the step is captured, not when it is replayed, and
 # no host code runs at a replay. Whatever is cached from such a parameter (arch/conv.py: _pver) is therefore keyed on a count that advances whenever
-# somebody asks for it from outside of a `fresh_params` call and of a backward pass, and once at the start of such a call.
+# somebody asks for it outside of a backward pass -- within a `fresh_params` call the first time only.
 graph_written = {}                                   # address of a storage -> count
-_in_fresh_params = [False]
+_fresh_seen = [None]                                 # the storages asked for in the running `fresh_params` call
 
 
 def note_graph_write(tensors) -> None:
@@ -491,24 +491,25 @@ def graph_write_count(t) -> int:
     n = graph_written.get(at)
     if n is None:
         return 0
-    if not _in_fresh_params[0] and graph_task_id() == -1:
+    seen = _fresh_seen[0]
+    if graph_task_id() == -1 and (seen is None or at not in seen):
         n = graph_written[at] = n + 1
+        if seen is not None:
+            seen.add(at)
     return n
 
 
 def fresh_params(method):
-    """Decorator of a module's method: within a call, what is cached from a parameter that replays write is made once, from the values at its start."""
+    """Decorator of a module's method: within a call, what is cached from a parameter that replays write is made once."""
     @functools.wraps(method)
     def call(self, *args, **kwargs):
-        if not graph_written or _in_fresh_params[0]:
+        if not graph_written or _fresh_seen[0] is not None:
             return method(self, *args, **kwargs)
-        for p in self.parameters():
-            graph_write_count(p)
-        _in_fresh_params[0] = True
+        _fresh_seen[0] = set()
         try:
             return method(self, *args, **kwargs)
         finally:
-            _in_fresh_params[0] = False
+            _fresh_seen[0] = None
     return call
 
 

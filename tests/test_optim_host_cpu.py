@@ -258,6 +258,29 @@ def test_checkpoints_follow_the_groups_as_they_are():
         opt.load_state_dict(sd)
 
 
+def test_a_module_within_another_ones_call_sees_its_own_replays(monkeypatch):
+    """A parameter that is first asked for inside of another module's `fresh_params` call has another version there than before."""
+    from nndetection_amd.arch.conv import _pver
+    monkeypatch.setattr(L, "graph_written", {})
+    w = torch.nn.Parameter(torch.zeros(3))
+    L.note_graph_write([w])
+
+    class Inner(torch.nn.Module):
+        @L.fresh_params
+        def forward(self):
+            return _pver(w)
+
+    inner = Inner()
+
+    class Outer(torch.nn.Module):
+        @L.fresh_params
+        def forward(self):
+            return inner(), inner(), _pver(w)
+
+    before, (a, b, c) = inner(), Outer()()
+    assert a == b == c != before
+
+
 def test_lists_of_a_derived_class(monkeypatch):
     ran = []
     monkeypatch.setattr(O, "_run", lambda *args: ran.append(args[1]))
