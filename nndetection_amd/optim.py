@@ -447,9 +447,10 @@ def _clip_call(grads, max_norm: float, grad_scale) -> torch.Tensor:
     _run(device, "nndet_grad_clip", words, n, max_norm, _scalar("grad_scale", grad_scale, device), norm.data_ptr())
     if max_norm >= 0.0:
         _written(flat)
-        for g, f in zip(grads, flat):
-            if f is not g:
-                g.copy_(f)
+        with torch.no_grad():
+            for g, f in zip(grads, flat):
+                if f is not g:
+                    g.copy_(f)
     return norm
 
 

@@ -295,3 +295,15 @@ def test_lists_of_a_derived_class(monkeypatch):
     O.write_adam_state8(st, m, v)
     O.read_adam_state8(st, m, v)
     assert len(ran) == 4
+
+
+def test_clipping_of_a_strided_leaf_that_requires_a_gradient(monkeypatch):
+    """Written back as it was computed, without a word to autograd: like the dense ones, and like torch's clipping."""
+    def scale(device, what, words, n, *args):
+        for t in (L.NndetOptTensor * n).from_buffer_copy(words):
+            (C.c_float * t.numel).from_address(t.grad)[:] = [3.0] * t.numel
+
+    monkeypatch.setattr(O, "_run", scale)
+    g = torch.zeros(4, 6)[:, ::2].requires_grad_()
+    O.clip_grads_([g], 1.0)
+    assert bool((g == 3).all()) and g.is_leaf
