@@ -88,6 +88,7 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         PyErr_SetString(PyExc_TypeError, "pack() takes 10 arguments");
         return nullptr;
     }
+    PyObject* out = nullptr;
     try {
         List p, g, m, v, ms, rs, wd;
         const bool listed = PyList_CheckExact(args[6]) || PyTuple_Check(args[6]);
@@ -99,7 +100,7 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const Py_ssize_t n = p.seq ? p.n : g.n;
         if ((!p.seq && !g.seq) || n >= (1 << 24) || (g.seq && g.n != n) || (m.seq && (!v.seq || m.n != n || v.n != n)) || (listed && wd.n != n)) Py_RETURN_NONE;
         if (ms.seq && (!rs.seq || ms.n != n || rs.n != n)) Py_RETURN_NONE;
-        PyObject* out = PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(NndetOptTensor));
+        out = PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(NndetOptTensor));
         if (!out) return nullptr;
         NndetOptTensor* t = reinterpret_cast<NndetOptTensor*>(PyBytes_AS_STRING(out));
         Addresses seen((p.seq ? 1 + (both != 0) : 1) * n + (m.seq ? 2 * n : 0) + (ms.seq ? 2 * n : 0));
@@ -167,7 +168,8 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     other:
         Py_DECREF(out);
         Py_RETURN_NONE;
-    } catch (const std::exception& e) {
+    } catch (const std::exception& e) {              // (a tensor without storage, as torch.func's wrappers are)
+        Py_XDECREF(out);
         PyErr_SetString(PyExc_RuntimeError, e.what());
         return nullptr;
     }

@@ -389,3 +389,25 @@ def test_three_rates_after_the_first_step(clip):
             within(p.detach(), wp[0], 1.5 * wp[1], what=str(i))
         assert opt._steps[ps[0].device].tolist() == [k + (i not in without) for i, k in enumerate(t)]
         assert opt.grad_norm is None if not clip else abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+
+
+def test_a_tensor_without_storage_leaves_nothing_behind():
+    """torch.func's wrappers have no address: the call raises, and frees what it had packed (500 structs of 72 bytes) until then."""
+    import tracemalloc
+    gs = [torch.zeros(1, device=DEV) for _ in range(500)]
+
+    def call(x):
+        with pytest.raises(RuntimeError):
+            O.grad_norm([*gs, x])
+        return x.sum()
+
+    x = torch.zeros(3, device=DEV)
+    torch.func.grad(call)(x)
+    tracemalloc.start()
+    try:
+        before = tracemalloc.get_traced_memory()[0]
+        for _ in range(20):
+            torch.func.grad(call)(x)
+        assert tracemalloc.get_traced_memory()[0] - before < 5 * 72 * 500
+    finally:
+        tracemalloc.stop()
